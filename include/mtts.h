@@ -303,6 +303,85 @@ int mtts_rope_table(float theta, int D, int n_pos, uint16_t* cos_host, uint16_t*
 int mtts_k_fill_uniform(uint16_t* dst, size_t n, uint64_t seed, uint64_t tensor_id, float scale, float offset,
                         void* stream);
 
+/* ---- drafted-token decoding over an 8-bit key / value cache ------------------------------------
+ * Rotary positions at explicit positions; a cache of bf16, e4m3 or int8 that new tokens are appended
+ * to, read back from and compacted in; attention of one token, a chain or a tree of drafted tokens
+ * over it.  All calls are asynchronous on `stream`, allocate nothing and may be captured into a
+ * graph; the caller's current device is the stream's.  Per-row numbers (start, counts, positions,
+ * paths, trees) are read on the device: a slot outside 0 .. slots-1 does not exist (nothing is
+ * written there or read from there), a count outside 0 .. T is taken as the nearer end. */
+#define MTTS_KV_BF16 0 /* K [rows][n_kv][slots][D], V transposed [rows][n_kv][D][slots]: the engine's layout */
+#define MTTS_KV_E4M3 1 /* one byte a value, one fp32 scale a (slot, head) for K and for V; 32-slot tiles (kvq.h) */
+#define MTTS_KV_INT8 2
+typedef struct mtts_kv_cache {
+  void *k, *v;              /* mtts_kv_bytes each, 16-byte aligned */
+  float *k_scale, *v_scale; /* [rows][n_kv][slots]; unused for MTTS_KV_BF16 */
+  int type, rows, n_kv, head_dim, slots; /* head_dim 32 / 64 / 128; slots a multiple of 32 */
+} mtts_kv_cache;
+/* bytes of k (and of v): the scales are rows * n_kv * slots floats each */
+size_t mtts_kv_bytes(int type, int rows, int n_kv, int head_dim, int slots);
+
+/* Rotation of the first rotary_dim dims of a head (even): pair i turns by position * turns[i]
+ * revolutions and is multiplied by factor.  Pairs are (i, i + rotary_dim / 2), or (2i, 2i + 1) when
+ * interleaved; the other dims pass through. */
+typedef struct mtts_rope {
+  const double* turns; /* device [rotary_dim / 2] */
+  int rotary_dim, interleaved;
+  float factor;
+} mtts_rope;
+#define MTTS_ROPE_DEFAULT 0
+#define MTTS_ROPE_LINEAR 1 /* frequencies / factor */
+#define MTTS_ROPE_NTK 2    /* base * factor^(d / (d - 2)) */
+#define MTTS_ROPE_YARN 3   /* by the turns a pair makes over the original length: interpolated, kept, or between */
+#define MTTS_ROPE_LLAMA3 4 /* the same by wavelength, linear between low_freq and high_freq turns */
+typedef struct mtts_rope_scaling {
+  int kind;
+  double factor, original_max_position; /* yarn, llama3 */
+  double beta_fast, beta_slow;          /* yarn (32, 1) */
+  double low_freq, high_freq;           /* llama3 (1, 4) */
+  double attention_factor;              /* yarn: <= 0 for 0.1 ln(factor) + 1 */
+} mtts_rope_scaling;
+/* host: turns_host[rotary_dim / 2] and the factor for a base and a scaling (NULL: none) */
+int mtts_rope_turns(double theta, int rotary_dim, const mtts_rope_scaling* scaling, double* turns_host, float* factor);
+/* y = rotated x: M tokens of H heads, ld* elements between tokens, hs* between heads; y may be x (with
+ * its strides).  pos_dev int32 [M].  head_dim even. */
+int mtts_k_rope(const uint16_t* x, size_t ldx, size_t hsx, uint16_t* y, size_t ldy, size_t hsy, const int32_t* pos_dev,
+                int M, int H, int head_dim, const mtts_rope* rope, void* stream);
+
+/* Appends S new tokens of rows 0 .. B-1: token t < counts[b] (NULL: S) of row b goes to slot
+ * start[b] + t.  q, k, v: token b * S + t at + (b * S + t) * ld, heads head_dim apart (the three may lie
+ * in one packed row).  k: RMSNorm over the head with weight kn_w (NULL: none), rotation (rope NULL:
+ * none) at pos_dev [B * S] (NULL: the slot), then quantised; v: quantised.  q (NULL: none): the same
+ * norm (qn_w) and rotation, to q_out in bf16; rows behind counts[b] are left as they are.
+ * A head's values are stored as code * scale, scale = max|x| / Q, code = nearest(x Q / max|x|), Q = 448
+ * (e4m3) or 127 (int8); a head below 2^-100 as zeros, one with a NaN or an infinity as NaN in whole. */
+int mtts_k_kv_append(const mtts_kv_cache* cache, const uint16_t* q, size_t ldq, const uint16_t* k, size_t ldk,
+                     const uint16_t* v, size_t ldv, uint16_t* q_out, size_t ldqo, int n_heads, const uint16_t* qn_w,
+                     const uint16_t* kn_w, float eps, const mtts_rope* rope, const int32_t* pos_dev,
+                     const int32_t* start_dev, const int32_t* counts_dev, int B, int S, void* stream);
+/* Slots start[b] (NULL: 0) .. + n - 1 of rows 0 .. B-1 as bf16 [B][n_kv][n][head_dim]; rows behind
+ * counts[b] (NULL: n) and slots past the cache's end are zeros. */
+int mtts_k_kv_read(const mtts_kv_cache* cache, uint16_t* k_out, uint16_t* v_out, const int32_t* start_dev,
+                   const int32_t* counts_dev, int B, int n, void* stream);
+/* The accepted path of a drafted tree: slot start[b] + i <- slot start[b] + path[b][i] for i < took[b]
+ * (all sources are read before any slot is written).  path int32 [B][P], P <= 64, entries 0 .. 63;
+ * an entry whose source is no slot is left out. */
+int mtts_k_kv_compact(const mtts_kv_cache* cache, const int32_t* start_dev, const int32_t* path_dev,
+                      const int32_t* took_dev, int B, int P, void* stream);
+/* Attention of T new tokens a row over its cache.  Token t < counts[b] (NULL: T) of row b sees the
+ * context slots j < start[b] with mask[b][j] != 0 (mask uint8 [B][slots], 8-byte aligned, NULL: all) and
+ * those new tokens u (slots start[b] + u) with bit u of tree[b][t] (T <= 64), or with tree NULL u <= t
+ * (any T).  softmax(scale q . k) v, scale <= 0: 1 / sqrt(head_dim).  A token that sees nothing gets
+ * zeros; what it does not see never reaches it, NaN and infinities included.  q / out: token b * T + t
+ * at + (b * T + t) * ld, [n_heads][head_dim]; rows behind counts[b] are left as they are.
+ * max_len: an upper bound of start the caller knows (<= 0: slots); it sizes the launch, not the result.
+ * ws_dev: mtts_k_attn_kv_ws_bytes bytes of scratch (0: NULL is fine), not shared by calls that may run
+ * at once; nothing is kept in it. */
+size_t mtts_k_attn_kv_ws_bytes(int B, int T, int n_heads, int n_kv, int head_dim, int slots, int max_len);
+int mtts_k_attn_kv(const mtts_kv_cache* cache, const uint16_t* q, size_t ldq, uint16_t* out, size_t ldo, int n_heads,
+                   const int32_t* start_dev, const int32_t* counts_dev, const uint64_t* tree_dev, const uint8_t* mask_dev,
+                   int B, int T, float scale, int max_len, void* ws_dev, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

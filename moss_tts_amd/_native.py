@@ -57,6 +57,22 @@ class MttsChannelSampling(ctypes.Structure):
                 ("top_p", ctypes.c_float), ("repetition_penalty", ctypes.c_float)]
 
 
+class MttsKvCache(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + \
+               [(n, ctypes.c_int) for n in ("type", "rows", "n_kv", "head_dim", "slots")]
+
+
+class MttsRope(ctypes.Structure):
+    _fields_ = [("turns", ctypes.c_void_p), ("rotary_dim", ctypes.c_int), ("interleaved", ctypes.c_int),
+                ("factor", ctypes.c_float)]
+
+
+class MttsRopeScaling(ctypes.Structure):
+    _fields_ = [("kind", ctypes.c_int)] + \
+               [(n, ctypes.c_double) for n in ("factor", "original_max_position", "beta_fast", "beta_slow", "low_freq",
+                                               "high_freq", "attention_factor")]
+
+
 P = ctypes.c_void_p
 I = ctypes.c_int
 F = ctypes.c_float
@@ -123,6 +139,15 @@ _SIGS = {
     "mtts_k_attn_decode": (I, [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, F, P]),
     "mtts_rope_table": (I, [F, I, I, P, P]),
     "mtts_k_fill_uniform": (I, [P, SZ, U64, U64, F, F, P]),
+    # drafted-token decoding over an 8-bit key / value cache
+    "mtts_kv_bytes": (SZ, [I, I, I, I, I]),
+    "mtts_rope_turns": (I, [ctypes.c_double, I, ctypes.POINTER(MttsRopeScaling), P, ctypes.POINTER(F)]),
+    "mtts_k_rope": (I, [P, SZ, SZ, P, SZ, SZ, P, I, I, I, P, P]),
+    "mtts_k_kv_append": (I, [P, P, SZ, P, SZ, P, SZ, P, SZ, I, P, P, F, P, P, P, P, I, I, P]),
+    "mtts_k_kv_read": (I, [P, P, P, P, P, I, I, P]),
+    "mtts_k_kv_compact": (I, [P, P, P, P, I, I, P]),
+    "mtts_k_attn_kv_ws_bytes": (SZ, [I, I, I, I, I, I, I]),
+    "mtts_k_attn_kv": (I, [P, P, SZ, P, SZ, I, P, P, P, P, I, I, F, I, P, P]),
     # codec decoder (include/mtts_codec.h)
     "mtts_codec_create": (I, [ctypes.POINTER(MttsCodecConfig), I, ctypes.POINTER(P)]),
     "mtts_codec_destroy": (I, [P]),

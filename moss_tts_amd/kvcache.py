@@ -1,0 +1,304 @@
+"""Drafted-token decoding over an 8-bit key / value cache: rotary positions, the cache, and the
+attention that reads it.
+
+    rope = Rope(128, theta=1e6, scaling={"rope_type": "yarn", "factor": 4.0,
+                                         "original_max_position_embeddings": 32768})
+    cache = KVCache(rows=4, n_kv=8, slots=8192, head_dim=128, dtype="e4m3")
+    q = cache.append(qkv, start, n_heads=32, rope=rope, positions=pos)   # norm, rotate, quantise, store
+    out = cache.attend(q, start, tree=masks)                             # verify a tree of drafted tokens
+    cache.compact(start, path, accepted)                                 # keep the accepted path
+
+Every call runs on the caller's current stream through libmtts.so (include/mtts.h), without a host
+synchronisation, and may be captured into a graph.  `start` (int32 [B], on the device) is the length
+of each row's context: new tokens take the slots behind it.  Rows and slots follow the engine's own
+cache: row b of a batch is row b of the cache.
+"""
+import ctypes
+from typing import List, Optional, Sequence, Tuple
+
+import torch
+
+from . import _native as N
+
+DTYPES = {"bf16": 0, "e4m3": 1, "int8": 2}
+TREE_MAX = 64
+
+_KINDS = {"default": 0, "linear": 1, "ntk": 2, "yarn": 3, "llama3": 4}
+
+
+def rope_turns(rotary_dim: int, theta: float, scaling: Optional[dict] = None) -> Tuple[torch.Tensor, float]:
+    """Host: (revolutions per position of each pair, float64 [rotary_dim / 2]; factor on the rotated
+    values).  `scaling` takes the keys of a model config's `rope_scaling` / `rope_parameters`:
+    rope_type default, linear, ntk, yarn or llama3; factor; original_max_position_embeddings;
+    beta_fast, beta_slow, attention_factor; low_freq_factor, high_freq_factor."""
+    sc = None
+    if scaling is not None:
+        kind = scaling.get("rope_type", scaling.get("type", "default"))
+        if kind not in _KINDS:
+            raise ValueError(f"rope_type {kind!r}: one of {sorted(_KINDS)}")
+        sc = N.MttsRopeScaling(_KINDS[kind], float(scaling.get("factor", 1.0)),
+                               float(scaling.get("original_max_position_embeddings", 0) or 0),
+                               float(scaling.get("beta_fast") or 32.0), float(scaling.get("beta_slow") or 1.0),
+                               float(scaling.get("low_freq_factor", 1.0)), float(scaling.get("high_freq_factor", 4.0)),
+                               float(scaling.get("attention_factor") or 0.0))
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError("rotary_dim is even and at least 2")
+    turns = torch.empty(rotary_dim // 2, dtype=torch.float64)
+    factor = ctypes.c_float()
+    N.call("mtts_rope_turns", float(theta), rotary_dim, None if sc is None else ctypes.byref(sc), turns.data_ptr(),
+           ctypes.byref(factor))
+    return turns, factor.value
+
+
+def _need(cond, what):
+    if not cond:
+        raise ValueError(what)
+
+
+class _On:
+    """the launches of a call go to the device that its tensors are on"""
+    __slots__ = ("dev",)
+
+    def __init__(self, index):
+        self.dev = None if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+    def __enter__(self):
+        if self.dev is not None:
+            self.dev.__enter__()
+
+    def __exit__(self, *e):
+        if self.dev is not None:
+            self.dev.__exit__(*e)
+
+
+def _device(device):
+    d = torch.device("cuda" if device is None else device)
+    if d.type != "cuda" or not torch.cuda.is_available():
+        raise RuntimeError("moss_tts_amd needs a ROCm GPU (MI355X); no CPU fallback exists")
+    return torch.device("cuda", torch.cuda.current_device() if d.index is None else d.index)
+
+
+class Rope:
+    """Rotary positions of `rotary_dim` (default: all) of a head's dims: half layout (pair i, i +
+    rotary_dim / 2) or interleaved (2i, 2i + 1), scaled as `rope_turns` says, or with explicit
+    frequencies `inv_freq` (radians per position) and `factor`."""
+
+    def __init__(self, head_dim: int, theta: float = 1e6, rotary_dim: Optional[int] = None, interleaved: bool = False,
+                 scaling: Optional[dict] = None, inv_freq: Optional[torch.Tensor] = None, factor: float = 1.0,
+                 device=None):
+        self.head_dim = head_dim
+        self.rotary_dim = head_dim if rotary_dim is None else rotary_dim
+        _need(head_dim >= 2 and head_dim % 2 == 0, "head_dim is even")
+        _need(2 <= self.rotary_dim <= head_dim and self.rotary_dim % 2 == 0, "rotary_dim is even and at most head_dim")
+        if inv_freq is None:
+            turns, self.factor = rope_turns(self.rotary_dim, theta, scaling)
+        else:
+            _need(scaling is None and inv_freq.numel() == self.rotary_dim // 2,
+                  "inv_freq holds rotary_dim / 2 frequencies, without a scaling")
+            turns, self.factor = inv_freq.detach().double().reshape(-1) / 6.283185307179586476925286766559, float(factor)
+        self.interleaved = bool(interleaved)
+        self.device = _device(device)
+        self.turns = turns.to(self.device).contiguous()
+        self._c = N.MttsRope(self.turns.data_ptr(), self.rotary_dim, int(self.interleaved), self.factor)
+        self._ref = ctypes.addressof(self._c)
+
+    def apply(self, x: torch.Tensor, positions: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """x bf16 [M, H, head_dim] (any strides between tokens and heads) at int32 positions [M];
+        `out` may be x itself."""
+        _need(x.dim() == 3 and x.dtype == torch.bfloat16 and x.shape[2] == self.head_dim and x.device == self.device,
+              "x is bf16 [tokens, heads, head_dim] on the frequencies' device")
+        M, H, D = x.shape
+        _i32(positions, (M,), self.device, "positions")
+        if out is None:
+            out = torch.empty((M, H, D), dtype=x.dtype, device=x.device)
+        else:
+            _need(out.shape == x.shape and out.dtype == x.dtype and out.device == x.device, "out is like x")
+        _need(x.stride(2) == 1 and out.stride(2) == 1, "a head's dims lie side by side")
+        with _On(self.device.index):
+            N.call("mtts_k_rope", x.data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+                   positions.data_ptr(), M, H, D, self._ref, _stream(self.device))
+        return out
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _i32(t, shape, device, what):
+    if t.dtype != torch.int32 or t.shape != shape or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{what}: contiguous int32 {list(shape)} on {device}")
+    return t.data_ptr()
+
+
+def tree_masks(parents: Sequence[Sequence[int]]) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Host: drafted trees as parents ([B][T]; -1: a root, else an earlier token) to (`tree` int64
+    [B, T] for `KVCache.attend`: bit u of entry t says that token t sees token u, its ancestors and
+    itself; depths int32 [B, T], to add to `start` for the positions)."""
+    masks: List[List[int]] = []
+    depths: List[List[int]] = []
+    for row in parents:
+        _need(len(row) <= TREE_MAX and len(row) == len(parents[0]), "trees of at most 64 tokens, padded to one length")
+        m: List[int] = []
+        d: List[int] = []
+        for t, p in enumerate(row):
+            _need(-1 <= p < t, "a token's parent comes before it")
+            m.append((m[p] if p >= 0 else 0) | 1 << t)
+            d.append(d[p] + 1 if p >= 0 else 0)
+        masks.append([x - (1 << 64) if x >> 63 else x for x in m])
+        depths.append(d)
+    return torch.tensor(masks, dtype=torch.int64), torch.tensor(depths, dtype=torch.int32)
+
+
+class KVCache:
+    """Keys and values of one layer: `rows` sequences of `slots` positions (rounded up to a multiple of
+    64), dtype "bf16" (the engine's layout: k [rows, n_kv, slots, D], v [rows, n_kv, D, slots]),
+    "e4m3" or "int8" (one byte a value in 32-slot tiles, one fp32 scale a slot and head)."""
+
+    def __init__(self, rows: int, n_kv: int, slots: int, head_dim: int, dtype: str = "e4m3", device=None):
+        _need(dtype in DTYPES, f"dtype: one of {sorted(DTYPES)}")
+        _need(rows > 0 and n_kv > 0 and slots > 0, "rows, heads and slots")
+        _need(head_dim in (32, 64, 128), "head_dim is 32, 64 or 128")
+        self.device = _device(device)
+        self.rows, self.n_kv, self.slots, self.head_dim, self.dtype = rows, n_kv, (slots + 63) // 64 * 64, head_dim, dtype
+        if dtype == "bf16":
+            self.k = torch.empty(rows, n_kv, self.slots, head_dim, dtype=torch.bfloat16, device=self.device)
+            self.v = torch.empty(rows, n_kv, head_dim, self.slots, dtype=torch.bfloat16, device=self.device)
+            self.k_scale = self.v_scale = None
+        else:
+            n = N.load().mtts_kv_bytes(DTYPES[dtype], rows, n_kv, head_dim, self.slots)
+            self.k = torch.empty(n, dtype=torch.uint8, device=self.device)
+            self.v = torch.empty(n, dtype=torch.uint8, device=self.device)
+            self.k_scale = torch.empty(rows, n_kv, self.slots, dtype=torch.float32, device=self.device)
+            self.v_scale = torch.empty_like(self.k_scale)
+        self._c = N.MttsKvCache(self.k.data_ptr(), self.v.data_ptr(),
+                                None if self.k_scale is None else self.k_scale.data_ptr(),
+                                None if self.v_scale is None else self.v_scale.data_ptr(), DTYPES[dtype], rows, n_kv,
+                                head_dim, self.slots)
+        self._ref = ctypes.addressof(self._c)
+
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale) if t is not None)
+
+    def _start(self, start, B):
+        _need(B <= self.rows, f"{B} rows for a cache of {self.rows}")
+        return _i32(start, (B,), self.device, "start")
+
+    def _counts(self, counts, B):
+        return None if counts is None else _i32(counts, (B,), self.device, "counts")
+
+    def _norm(self, w, what):
+        if w is None:
+            return None
+        _need(w.dtype == torch.bfloat16 and w.shape == (self.head_dim,) and w.is_contiguous() and w.device == self.device,
+              f"{what}: bf16 [head_dim]")
+        return w.data_ptr()
+
+    def _append(self, q, k, v, out, n_heads, ld, B, S, start, rope, positions, counts, q_norm, k_norm, eps):
+        if rope is not None:
+            _need(rope.head_dim == self.head_dim and rope.device == self.device, "rope is of another head or device")
+        with _On(self.device.index):
+            N.call("mtts_k_kv_append", self._ref, q, ld[0], k, ld[1], v, ld[2],
+                   None if out is None else out.data_ptr(), n_heads * self.head_dim, n_heads,
+                   self._norm(q_norm, "q_norm"), self._norm(k_norm, "k_norm"), eps, None if rope is None else rope._ref,
+                   None if positions is None else _i32(positions, (B, S), self.device, "positions"),
+                   self._start(start, B), self._counts(counts, B), B, S, _stream(self.device))
+
+    def append(self, qkv: torch.Tensor, start: torch.Tensor, n_heads: int, rope: Optional[Rope] = None,
+               positions: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None,
+               q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """qkv bf16 [B, S, (n_heads + 2 n_kv) * head_dim], the output of the q|k|v projection: norms and
+        rotates q and k (positions int32 [B, S]; None: the slots), stores k and v at slots start[b] ..,
+        returns q [B, S, n_heads, head_dim].  Rows behind counts[b] (int32 [B]; None: S) store nothing;
+        their q is zero, or what `out` held."""
+        D = self.head_dim
+        _need(qkv.dim() == 3 and qkv.dtype == torch.bfloat16 and qkv.device == self.device and
+              n_heads > 0 and qkv.shape[2] == (n_heads + 2 * self.n_kv) * D, "qkv: bf16 [B, S, (n_heads + 2 n_kv) * head_dim]")
+        B, S, _ = qkv.shape
+        ld = qkv.stride(1) if S > 1 else qkv.stride(0)
+        _need(qkv.stride(2) == 1 and (B <= 1 or S <= 1 or qkv.stride(0) == S * qkv.stride(1)), "qkv: rows one stride apart")
+        if out is None:
+            out = (torch.empty if counts is None else torch.zeros)((B, S, n_heads, D), dtype=torch.bfloat16,
+                                                                  device=self.device)
+        else:
+            _need(out.shape == (B, S, n_heads, D) and out.dtype == torch.bfloat16 and out.is_contiguous() and
+                  out.device == self.device, "out: contiguous bf16 [B, S, n_heads, head_dim]")
+        p = qkv.data_ptr()
+        self._append(p, p + 2 * n_heads * D, p + 2 * (n_heads + self.n_kv) * D, out, n_heads, (ld, ld, ld), B, S, start,
+                     rope, positions, counts, q_norm, k_norm, eps)
+        return out
+
+    def write(self, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor, rope: Optional[Rope] = None,
+              positions: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None) -> None:
+        """k, v bf16 [B, S, n_kv, head_dim]: stored at slots start[b] .. (k rotated if `rope` is given)."""
+        lds = []
+        B, S = k.shape[:2]
+        for t in (k, v):
+            _need(t.dim() == 4 and t.dtype == torch.bfloat16 and t.device == self.device and
+                  t.shape == (B, S, self.n_kv, self.head_dim), "k, v: bf16 [B, S, n_kv, head_dim]")
+            ld = t.stride(1) if S > 1 else t.stride(0)
+            _need(t.stride(3) == 1 and (self.n_kv == 1 or t.stride(2) == self.head_dim) and
+                  (B <= 1 or S <= 1 or t.stride(0) == S * t.stride(1)), "k, v: heads side by side, rows one stride apart")
+            lds.append(ld)
+        self._append(None, k.data_ptr(), v.data_ptr(), None, 0, (0, *lds), B, S, start, rope, positions, counts, None, None,
+                     0.0)
+
+    def read(self, n: int, start: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None,
+             rows: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Slots start[b] (None: 0) .. + n - 1 of the first `rows` rows (default: start's, or all) as bf16
+        (k, v), each [rows, n_kv, n, head_dim]; rows behind counts[b] and slots past the end are zeros."""
+        B = rows if rows is not None else self.rows if start is None else start.shape[0]
+        _need(n >= 0 and B >= 0, "read: sizes")
+        _need(B <= self.rows, f"{B} rows for a cache of {self.rows}")
+        k = torch.empty((B, self.n_kv, n, self.head_dim), dtype=torch.bfloat16, device=self.device)
+        v = torch.empty_like(k)
+        with _On(self.device.index):
+            N.call("mtts_k_kv_read", self._ref, k.data_ptr(), v.data_ptr(), None if start is None else self._start(start, B),
+                   self._counts(counts, B), B, n, _stream(self.device))
+        return k, v
+
+    def compact(self, start: torch.Tensor, path: torch.Tensor, accepted: torch.Tensor) -> None:
+        """Keeps the accepted path of a drafted tree: slot start[b] + i takes what slot start[b] +
+        path[b, i] holds, for i < accepted[b] (path int32 [B, P], P <= 64; accepted int32 [B])."""
+        _need(path.dim() == 2, "path: int32 [B, P]")
+        B, P = path.shape
+        with _On(self.device.index):
+            N.call("mtts_k_kv_compact", self._ref, self._start(start, B), _i32(path, (B, P), self.device, "path"),
+                   _i32(accepted, (B,), self.device, "accepted"), B, P, _stream(self.device))
+
+    def attend(self, q: torch.Tensor, start: torch.Tensor, tree: Optional[torch.Tensor] = None,
+               counts: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+               max_len: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """q bf16 [B, T, n_heads, head_dim] of tokens whose keys stand in slots start[b] .. (appended
+        before): softmax(scale q . k) v over the context slots that mask (uint8 / bool [B, slots], 1 =
+        attend) keeps and the new tokens that tree (int64 [B, T], `tree_masks`; None: a chain) shows.
+        A token that sees nothing gets zeros; rows behind counts[b] are zero, or what `out` held.
+        max_len: an upper bound of `start` known to the caller, for the shape of the launch only."""
+        _need(q.dim() == 4 and q.dtype == torch.bfloat16 and q.shape[3] == self.head_dim and q.device == self.device,
+              "q: bf16 [B, T, n_heads, head_dim]")
+        B, T, H, D = q.shape
+        ldq = q.stride(1) if T > 1 else q.stride(0)
+        _need(q.stride(3) == 1 and (H == 1 or q.stride(2) == D) and (B <= 1 or T <= 1 or q.stride(0) == T * q.stride(1)),
+              "q: heads side by side, rows one stride apart")
+        if tree is not None:
+            _need(tree.dtype == torch.int64 and tree.shape == (B, T) and tree.is_contiguous() and
+                  tree.device == self.device, "tree: contiguous int64 [B, T]")
+        if mask is not None:
+            _need(mask.dtype in (torch.uint8, torch.bool) and mask.shape == (B, self.slots) and mask.is_contiguous() and
+                  mask.device == self.device, f"mask: contiguous uint8 [B, {self.slots}]")
+        if out is None:
+            out = (torch.empty if counts is None else torch.zeros)((B, T, H, D), dtype=torch.bfloat16, device=self.device)
+        else:
+            _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous() and out.device == self.device,
+                  "out: contiguous, like q")
+        _need(scale is None or scale > 0, "scale > 0")
+        n = 0 if max_len is None else max(1, int(max_len))
+        L = N.load()
+        with _On(self.device.index):
+            need = L.mtts_k_attn_kv_ws_bytes(B, T, H, self.n_kv, D, self.slots, n)
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+            N.check(L.mtts_k_attn_kv(self._ref, q.data_ptr(), ldq, out.data_ptr(), H * D, H, self._start(start, B),
+                                     self._counts(counts, B), None if tree is None else tree.data_ptr(),
+                                     None if mask is None else mask.data_ptr(), B, T, 0.0 if scale is None else scale, n,
+                                     None if ws is None else ws.data_ptr(), _stream(self.device)), "attend")
+        return out

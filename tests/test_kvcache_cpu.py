@@ -1,0 +1,195 @@
+"""Drafted-token operators, host side: rotary frequencies against their formulas, tree masks, and the
+refusals of the C entry points (every check comes before any device call)."""
+import ctypes
+import math
+import os
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module")
+def kv():
+    from moss_tts_amd import _native, kvcache
+    if not os.path.exists(_native.lib_path()):
+        pytest.skip("libmtts.so not built")
+    _native.load()
+    return kvcache
+
+
+@pytest.fixture(scope="module")
+def N(kv):
+    from moss_tts_amd import _native
+    return _native
+
+
+def formula(rot, theta, sc):
+    """radians per position, from the definitions"""
+    f = [theta ** (-2.0 * i / rot) for i in range(rot // 2)]
+    kind = sc.get("rope_type", "default")
+    s = sc.get("factor", 1.0)
+    if kind == "linear":
+        return [x / s for x in f], 1.0
+    if kind == "ntk":
+        return [(theta * s ** (rot / (rot - 2.0))) ** (-2.0 * i / rot) for i in range(rot // 2)], 1.0
+    if kind == "default":
+        return f, 1.0
+    old = sc["original_max_position_embeddings"]
+    if kind == "llama3":
+        lo, hi = sc.get("low_freq_factor", 1.0), sc.get("high_freq_factor", 4.0)
+        out = []
+        for x in f:
+            turns = old * x / (2 * math.pi)
+            w = (turns - lo) / (hi - lo)
+            out.append(x / s if turns < lo else x if turns > hi else (1 - w) * x / s + w * x)
+        return out, 1.0
+    at = lambda b: rot * math.log(old / (b * 2 * math.pi)) / (2 * math.log(theta))  # noqa: E731
+    lo, hi = max(math.floor(at(sc.get("beta_fast", 32))), 0), min(math.ceil(at(sc.get("beta_slow", 1))), rot - 1)
+    hi = hi + 0.001 if hi == lo else hi
+    out = []
+    for i, x in enumerate(f):
+        r = min(1.0, max(0.0, (i - lo) / (hi - lo)))
+        out.append(x / s * r + x * (1 - r))
+    return out, sc.get("attention_factor", 0.1 * math.log(s) + 1.0)
+
+
+@pytest.mark.parametrize("rot", [2, 10, 64, 128])
+@pytest.mark.parametrize("sc", [{}, dict(rope_type="linear", factor=4.0), dict(rope_type="ntk", factor=8.0),
+                                dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=32768),
+                                dict(rope_type="yarn", factor=16.0, original_max_position_embeddings=4096, beta_fast=24,
+                                     beta_slow=2, attention_factor=1.5),
+                                dict(rope_type="llama3", factor=8.0, low_freq_factor=1.0, high_freq_factor=4.0,
+                                     original_max_position_embeddings=8192)])
+def test_rope_turns(kv, rot, sc):
+    if sc.get("rope_type") == "ntk" and rot == 2:
+        pytest.skip("refused, below")
+    turns, factor = kv.rope_turns(rot, 1e6, sc or None)
+    want, m = formula(rot, 1e6, sc)
+    got = turns * 2 * math.pi
+    # 64-bit powers and logarithms: a few steps of 2^-53
+    assert torch.allclose(got, torch.tensor(want, dtype=torch.float64), rtol=1e-13, atol=0)
+    assert abs(factor - m) <= 2.0 ** -24 * m
+
+
+@pytest.mark.parametrize("rot,theta,sc", [(3, 1e4, None), (0, 1e4, None), (64, 1.0, None), (64, float("nan"), None),
+                                          (64, 1e4, dict(rope_type="linear", factor=0.5)),
+                                          (64, 1e4, dict(rope_type="yarn", factor=4.0)),
+                                          (64, 1e4, dict(rope_type="llama3", factor=8.0, low_freq_factor=4.0,
+                                                         high_freq_factor=4.0, original_max_position_embeddings=8192)),
+                                          (2, 1e4, dict(rope_type="ntk", factor=2.0)),
+                                          (64, 1e4, dict(rope_type="longer"))])
+def test_rope_turns_refusals(kv, rot, theta, sc):
+    with pytest.raises(ValueError):
+        kv.rope_turns(rot, theta, sc)
+
+
+def test_tree_masks(kv):
+    masks, depth = kv.tree_masks([[-1, 0, 0, 1, 3], [-1, -1, 1, 2, 0]])
+    assert masks.tolist() == [[1, 3, 5, 11, 27], [1, 2, 6, 14, 17]]
+    assert depth.tolist() == [[0, 1, 1, 2, 3], [0, 0, 1, 2, 1]] and depth.dtype == torch.int32
+    chain, _ = kv.tree_masks([list(range(-1, 63))])
+    assert chain[0, 63].item() == -1 and chain[0, 62].item() == (1 << 63) - 1
+    for bad in ([[0]], [[-1, 2]], [[-1], [-1, 0]], [[-1] + list(range(64))]):
+        with pytest.raises(ValueError):
+            kv.tree_masks(bad)
+
+
+FAKE = 1 << 20  # an aligned address that no check follows
+
+
+def cache(N, **kw):
+    f = dict(k=FAKE, v=FAKE, k_scale=FAKE, v_scale=FAKE, type=1, rows=2, n_kv=2, head_dim=64, slots=64)
+    f.update(kw)
+    return N.MttsKvCache(*(f[n] for n, _ in N.MttsKvCache._fields_))
+
+
+BAD_CACHES = [dict(k=None), dict(v=None), dict(k_scale=None), dict(type=3), dict(type=-1), dict(rows=0), dict(n_kv=0),
+              dict(slots=0), dict(slots=48), dict(k=FAKE + 8), dict(v_scale=FAKE + 4)]
+
+
+@pytest.mark.parametrize("bad", BAD_CACHES)
+def test_bad_caches(N, bad):
+    c = ctypes.byref(cache(N, **bad))
+    with pytest.raises(ValueError):
+        N.call("mtts_k_kv_append", c, None, 0, FAKE, 128, FAKE, 128, None, 0, 0, None, None, 0.0, None, None, FAKE, None, 1, 1,
+               None)
+    with pytest.raises(ValueError):
+        N.call("mtts_k_kv_read", c, FAKE, FAKE, None, None, 1, 1, None)
+    with pytest.raises(ValueError):
+        N.call("mtts_k_kv_compact", c, FAKE, FAKE, FAKE, 1, 1, None)
+    with pytest.raises(ValueError):
+        N.call("mtts_k_attn_kv", c, FAKE, 256, FAKE, 256, 4, FAKE, None, None, None, 1, 1, 0.0, 0, FAKE, None)
+
+
+@pytest.mark.parametrize("D", [16, 96, 256])
+def test_head_dims_refused(N, D):
+    with pytest.raises(RuntimeError, match="head_dim"):
+        N.call("mtts_k_attn_kv", ctypes.byref(cache(N, head_dim=D)), FAKE, 4 * D, FAKE, 4 * D, 4, FAKE, None, None, None, 1, 1,
+               0.0, 0, FAKE, None)
+
+
+def test_attention_refusals(N):
+    c = ctypes.byref(cache(N))
+    ok = dict(q=FAKE, ldq=256, out=FAKE, ldo=256, H=4, start=FAKE, counts=None, tree=None, mask=None, B=1, T=1, scale=0.0,
+              max_len=0, ws=FAKE)
+
+    def call(**kw):
+        N.call("mtts_k_attn_kv", c, *{**ok, **kw}.values(), None)
+    for bad in (dict(q=None), dict(out=None), dict(start=None), dict(H=3), dict(H=0), dict(B=3), dict(B=-1), dict(T=-1),
+                dict(q=FAKE + 2), dict(ldq=260), dict(out=FAKE + 4), dict(ldo=258), dict(mask=FAKE + 4), dict(ws=FAKE + 8)):
+        with pytest.raises(ValueError):
+            call(**bad)
+    with pytest.raises(RuntimeError, match="at most 64"):
+        call(T=65, tree=FAKE)
+    long = ctypes.byref(cache(N, slots=8192))
+    assert N.load().mtts_k_attn_kv_ws_bytes(1, 1, 4, 2, 64, 8192, 0) > 0
+    with pytest.raises(ValueError, match="workspace"):
+        N.call("mtts_k_attn_kv", long, *{**ok, "ws": None}.values(), None)
+    call(B=0), call(T=0)  # nothing to do: no launch
+
+
+def test_append_and_move_refusals(N):
+    c = ctypes.byref(cache(N))
+    rope = N.MttsRope(FAKE, 64, 0, 1.0)
+
+    def app(q=None, k=FAKE, v=FAKE, q_out=None, H=0, rope=None, start=FAKE, B=1, S=1):
+        N.call("mtts_k_kv_append", c, q, 256, k, 128, v, 128, q_out, 256, H, None, None, 0.0,
+               None if rope is None else ctypes.byref(rope), None, start, None, B, S, None)
+    for bad in (dict(k=None), dict(v=None), dict(start=None), dict(q=FAKE, H=4), dict(q=FAKE, q_out=FAKE), dict(B=3),
+                dict(S=-1), dict(rope=N.MttsRope(FAKE, 66, 0, 1.0)), dict(rope=N.MttsRope(FAKE, 3, 0, 1.0)),
+                dict(rope=N.MttsRope(None, 64, 0, 1.0))):
+        with pytest.raises(ValueError):
+            app(**bad)
+    app(B=0), app(S=0)
+    for bad in ((None, FAKE, None, None, 1, 1), (FAKE, FAKE + 8, None, None, 1, 1), (FAKE, FAKE, None, None, 3, 1),
+                (FAKE, FAKE, None, None, 1, -1)):
+        with pytest.raises(ValueError):
+            N.call("mtts_k_kv_read", c, *bad, None)
+    for bad in ((None, FAKE, FAKE, 1, 1), (FAKE, None, FAKE, 1, 1), (FAKE, FAKE, None, 1, 1), (FAKE, FAKE, FAKE, 3, 1)):
+        with pytest.raises(ValueError):
+            N.call("mtts_k_kv_compact", c, *bad, None)
+    with pytest.raises(RuntimeError, match="at most 64"):
+        N.call("mtts_k_kv_compact", c, FAKE, FAKE, FAKE, 1, 65, None)
+    for bad in (dict(x=None), dict(pos=None), dict(D=63), dict(M=-1), dict(ldy=256), dict(hs=32), dict(rope=None)):
+        f = dict(x=FAKE, ldx=128, hs=64, ldy=128, pos=FAKE, M=2, D=64, rope=ctypes.byref(rope))
+        f.update(bad)
+        with pytest.raises(ValueError):
+            N.call("mtts_k_rope", f["x"], f["ldx"], f["hs"], FAKE, f["ldy"], f["hs"], f["pos"], f["M"], 2, f["D"], f["rope"],
+                   None)
+
+
+def test_workspace_bytes(N):
+    L = N.load()
+    assert L.mtts_k_attn_kv_ws_bytes(64, 64, 32, 8, 128, 2048, 0) == 0  # one block a row and KV head: no partials
+    one = L.mtts_k_attn_kv_ws_bytes(1, 1, 32, 8, 128, 131072, 0)
+    assert one > 0 and L.mtts_k_attn_kv_ws_bytes(1, 1, 32, 8, 128, 131072, 100) == 0 and one % 4 == 0
+    assert L.mtts_kv_bytes(0, 2, 8, 128, 4096) == 2 * L.mtts_kv_bytes(1, 2, 8, 128, 4096) == 2 * 2 * 8 * 128 * 4096
+
+
+def test_layout_is_a_permutation(kv):
+    """the tile layout as the header states it: every (slot, dim) has a byte of its own"""
+    for D in (32, 64, 128):
+        from tests.kv_layout import k_bytes, v_bytes
+        for f in (k_bytes, v_bytes):
+            assert sorted(f(D).reshape(-1).tolist()) == list(range(32 * D))
