@@ -12,8 +12,11 @@
 //   O^T [D x 32 rows] += V^T . P^T
 // The score tile's row order is chosen so that a lane's 16 scores are those of slots 16 u + 8 h + i
 // (h = lane / 32): exactly the operand that the second product wants from that lane, so the
-// probabilities never leave its registers, and K / V fragments come straight from memory: no LDS in
-// the loop and no barrier.  The 4 waves of a block take tiles in turn and merge once at the end.
+// probabilities never leave its registers.
+//   The running maximum lives in powers of two: p = 2^(s scale log2(e) - m).  A slot's two scales are
+// held one a lane and reach the 16 scores as row broadcasts, an operand form that costs nothing.
+#include <utility>
+
 #include "engine_internal.h"
 #include "kvq.h"
 
@@ -34,56 +37,72 @@ __device__ __forceinline__ RowLen row_len(const AttnKvArgs& a, int b) {
   return r;
 }
 
-// Splits.  NS blocks (a KV head and row block each) are shared out over the batch's rows by their
-// lengths, which only the device knows: row b gets 1 + (NS - B) nt_b / sum(nt), at most one for each
-// 4 tiles.  Every block works the table out for itself (one wave-wide scan of the lengths).
-struct Split {
-  int b, s, ns, x0;
-};
-__device__ __forceinline__ int splits_of(int nt, int total, int extra) {
-  const int want = total > 0 ? 1 + (int)((int64_t)extra * nt / total) : 1;
-  return max(1, min(want, (nt + 3) / 4));
+// Work.  The batch's rows differ in length and only the device knows by how much, so the blocks of a KV
+// head (and row block) share out the tiles of all rows as one run: block x takes tiles x share ..
+// (x + 1) share - 1 of it, in segments of one row each.  A row that lies in one block is finished there;
+// of a longer one every block leaves a partial (m, l, o), in slot 2 x + 1 if the row begins in it and
+// 2 x if it began before, and the join adds them up in order: the first block and the number of blocks of
+// each row stand at the head of the workspace.  share 0: a block a row, nothing to join.
+__device__ __forceinline__ int tiles_of(const RowLen& r) { return r.n ? (r.nk + 31) >> 5 : 0; }
+__device__ __forceinline__ int wave_isum(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return __builtin_amdgcn_readfirstlane(v);
 }
-// the split with number x (b = -1: none), or with x < 0 row `row`'s first
-__device__ Split find_split(const AttnKvArgs& a, int NS, int x, int row) {
-  Split r{-1, 0, 1, 0};
-  if (NS == a.B) {
-    r.b = x < 0 ? row : x;
-    r.x0 = r.b;
-    return r;
+__device__ __forceinline__ int wave_iscan(int v, int lane) {  // sum up to and with this lane
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(v, o, 64);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+struct Seg {
+  int b, t0, t1, slot;  // tiles [t0, t1) of row b; slot -1: the whole row
+  RowLen len;
+};
+template <class F>
+__device__ __forceinline__ void for_segments(const AttnKvArgs& a, int NS, int least, int x, bool head, F&& body) {
+  if (least == 0) {
+    const RowLen r = row_len(a, x);
+    body(Seg{x, 0, INT_MAX, -1, r});
+    return;
   }
   const int lane = threadIdx.x & 63;
-  int total = 0, nt = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    nt = b0 + lane < a.B ? (row_len(a, b0 + lane).nk + 31) >> 5 : 0;
-    int t = nt;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
-    total += t;
+  int total = 0;
+  RowLen r{0, 0, 0};
+  for (int b0 = (a.B - 1) & ~63; b0 >= 0; b0 -= 64) {
+    r = b0 + lane < a.B ? row_len(a, b0 + lane) : RowLen{0, 0, 0};
+    total += wave_isum(tiles_of(r));
   }
+  const int share = max(least, (total + NS - 1) / NS);
+  const int64_t lo = (int64_t)x * share, hi = lo + share;
   int off = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    if (a.B > 64) nt = b0 + lane < a.B ? (row_len(a, b0 + lane).nk + 31) >> 5 : 0;
-    const int ns = b0 + lane < a.B ? splits_of(nt, total, NS - a.B) : 0;
-    int incl = ns;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int v = __shfl_up(incl, o, 64);
-      if (lane >= o) incl += v;
+  for (int b0 = 0; b0 < a.B && (off < hi || head); b0 += 64) {
+    if (b0) r = b0 + lane < a.B ? row_len(a, b0 + lane) : RowLen{0, 0, 0};
+    const int nt = tiles_of(r), end = off + wave_iscan(nt, lane), beg = end - nt;
+    if (head && threadIdx.x < 64 && b0 + lane < a.B) {
+      const int x0 = nt ? beg / share : 0, ns = nt ? (end - 1) / share - x0 + 1 : 0;
+      *reinterpret_cast<int2*>(a.part + 2 * (b0 + lane)) = make_int2(x0, ns);
     }
-    const uint64_t hit = __ballot(x < 0 ? b0 + lane == row : ns > 0 && x < off + incl);
-    if (hit) {
+    uint64_t hit = __ballot(nt > 0 && beg < hi && end > lo);
+    while (hit) {
       const int f = __ffsll((unsigned long long)hit) - 1;
-      r.b = b0 + f;
-      r.ns = __builtin_amdgcn_readfirstlane(__shfl(ns, f, 64));
-      r.x0 = __builtin_amdgcn_readfirstlane(off + __shfl(incl, f, 64)) - r.ns;
-      r.s = x - r.x0;
-      return r;
+      hit &= hit - 1;
+      const int sb = __builtin_amdgcn_readlane(beg, f), se = __builtin_amdgcn_readlane(end, f);
+      Seg g;
+      g.b = b0 + f;
+      g.t0 = (int)max(lo, (int64_t)sb) - sb;
+      g.t1 = (int)min(hi, (int64_t)se) - sb;
+      g.slot = sb >= lo && se <= hi ? -1 : 2 * x + (sb >= lo ? 1 : 0);
+      g.len = RowLen{__builtin_amdgcn_readlane(r.start, f), __builtin_amdgcn_readlane(r.n, f), __builtin_amdgcn_readlane(r.nk, f)};
+      body(g);
     }
-    off += __builtin_amdgcn_readfirstlane(__shfl(incl, 63, 64));
+    off = __builtin_amdgcn_readlane(end, 63);
   }
-  return r;
 }
+// floats at the head of the workspace
+__host__ __device__ __forceinline__ size_t head_floats(int B) { return ((size_t)2 * B + 63) / 64 * 64; }
 
 // eight codes as bf16: exact, both types have at most 8 significant bits
 template <int KT>
@@ -102,457 +121,824 @@ __device__ __forceinline__ bf16x8 frag8(uint32_t lo, uint32_t hi) {
     const uint32_t w[2] = {lo, hi};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float x = (float)(int8_t)(w[i >> 1] >> (16 * (i & 1)));
-      const float y = (float)(int8_t)(w[i >> 1] >> (16 * (i & 1) + 8));
+      const float x = (float)(int)__builtin_amdgcn_sbfe(w[i >> 1], 16 * (i & 1), 8);
+      const float y = (float)(int)__builtin_amdgcn_sbfe(w[i >> 1], 16 * (i & 1) + 8, 8);
       o.w[i] = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302);  // the high halves
     }
   }
   return o.v;
 }
 
-template <int KT, int D, int RT>
-__global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void attn_kv_kernel(AttnKvArgs a, int NS, int RB) {
+// compile-time unrolled: the lane of a row broadcast is part of the instruction
+template <int N, class F, int... I>
+__device__ __forceinline__ void unrolled_impl(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void unrolled(F&& f) {
+  unrolled_impl<N>(f, std::make_integer_sequence<int, N>{});
+}
+// lane i's value of each row of 16 lanes, in all of the row
+template <int I>
+__device__ __forceinline__ float row_bcast(float v) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x150 + I, 0xf, 0xf, true));
+}
+
+// Of the 8 slots from k0 on (bits): live, the context slots that the mask keeps and the new tokens'
+// (every other slot's bytes are anything); fresh, the new tokens' alone.
+struct Live8 {
+  uint32_t live, fresh;
+};
+__device__ __forceinline__ Live8 live8(const AttnKvArgs& a, int b, const RowLen& len, int k0) {
+  const int cn = min(max(len.start - k0, 0), 8), ln = min(max(len.nk - k0, 0), 8);
+  uint32_t ctx = (1u << cn) - 1;
+  const uint32_t fresh = ((1u << ln) - 1) & ~ctx;
+  if (a.mask) {
+    const uint2 mk = *reinterpret_cast<const uint2*>(a.mask + (size_t)b * a.c.slots + k0);
+    uint32_t mb = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      mb |= ((mk.x >> (8 * i)) & 0xff ? 1u << i : 0) | ((mk.y >> (8 * i)) & 0xff ? 16u << i : 0);
+    ctx &= mb;
+  }
+  return {ctx | fresh, fresh};
+}
+
+// A lane's row: its token and, for a tree, what the token sees.
+struct Row {
+  int tok;
+  uint64_t tw;
+};
+// the 16 slots of lane half h in a tile that may hold slots the row does not see: bit 8 u + i for slot
+// 16 u + 8 h + i; live as above
+__device__ __forceinline__ void edge_bits(const AttnKvArgs& a, int b, const RowLen& len, int tile, int h, const Row& row,
+                                          uint32_t* live, uint32_t* sees) {
+  *live = *sees = 0;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int k0 = tile * 32 + 16 * u + 8 * h, d0 = k0 - len.start;  // d0: the new token of the first slot
+    const Live8 l = live8(a, b, len, k0);
+    uint32_t w;
+    if (a.tree) w = d0 >= 0 ? (d0 < 64 ? (uint32_t)(row.tw >> d0) : 0) : d0 > -8 ? (uint32_t)row.tw << -d0 : 0;
+    else w = (1u << min(max(row.tok + 1 - d0, 0), 8)) - 1;
+    *live |= l.live << (8 * u);
+    *sees |= ((l.live & ~l.fresh) | (l.fresh & w)) << (8 * u);
+  }
+}
+
+// a value fragment whose slots are dead: zero, whatever the bytes are
+template <int KT>
+__device__ __forceinline__ u32x4 clear_dead(u32x4 f, uint32_t live) {  // 8-bit: 16 slots; bf16: 8
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t w = f[i];
+    if constexpr (KT == KV_BF16) {
+      w &= (live >> (2 * i) & 1 ? 0xffffu : 0) | (live >> (2 * i + 1) & 1 ? 0xffff0000u : 0);
+    } else {
+      uint32_t keep = 0;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) keep |= live >> (4 * i + y) & 1 ? 0xffu << (8 * y) : 0;
+      w &= keep;
+      if constexpr (KT == KV_E4M3) {
+        // (append writes no NaN code, a NaN row has a NaN scale; a new token's slot that was never
+        // written may hold one, and rows that do not see it are spared)
+        const uint32_t nan = (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+        w &= ~(nan * 0xffu);
+      }
+    }
+    f[i] = w;
+  }
+  return f;
+}
+
+// the larger of the two lane halves' values, in both
+__device__ __forceinline__ float half_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// One row tile's running softmax and output, 32 rows a wave (lane n = lane % 32's row).
+template <int KT, int D>
+struct RowState {
+  static constexpr int DT = D / 32;
+  f32x16 o[DT];
+  float m, l;
+
+  __device__ __forceinline__ void clear() {
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
+  }
+
+  // Scores to probabilities in two parts, so that the second can stand beside other products.
+  // scores: s raw products, c = scale log2(e), kcl = c times this lane's slot's key scale (8-bit types).
+  __device__ __forceinline__ void scores(f32x16& s, float c, float kcl, bool edge, uint32_t sees) {
+    if constexpr (KT != KV_BF16) unrolled<16>([&](auto i) { s[i.value] *= row_bcast<i.value>(kcl); });
+    if (edge) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = sees >> i & 1 ? s[i] : -INFINITY;
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+    mx = half_max(mx);
+    if constexpr (KT == KV_BF16) mx *= c;
+    // m follows the maximum only once that has outgrown it by 2^8: p stays below 256, which costs no bit of
+    // it, and the 16 D / 32 products of the output's rescaling are rare (at each new maximum of any of 32
+    // rows they were two fifths of the loop)
+    if (__any(mx > m + 8.f)) {
+      const float mn = fmaxf(m, mx);
+      const float al = m == -INFINITY ? (mn == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= al;
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[t][i] *= al;
+    }
+  }
+  // probs: vsl this lane's slot's value scale.  p: the operand of the second product.  p is rounded to bf16,
+  // the product's type: half a step of 2^-8 at random signs over the keys, no more than the output's own
+  // rounding; sums stay in 32 bits.
+  __device__ __forceinline__ void probs(const f32x16& s, float c, float vsl, uint32_t sees, bool special, bf16x8* p) {
+    constexpr bool Q8 = KT != KV_BF16;
+    const float mu = m == -INFINITY ? 0.f : m;
+    float e[16], sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      e[i] = __builtin_amdgcn_exp2f(Q8 ? s[i] - mu : fmaf(s[i], c, -mu));
+      sum += e[i];
+    }
+    l += sum;
+    if constexpr (Q8) {
+      unrolled<16>([&](auto i) { e[i.value] *= row_bcast<i.value>(vsl); });
+      if (special) {  // some slot's scale is not finite: it counts for the rows that see it alone
+#pragma unroll
+        for (int i = 0; i < 16; ++i) e[i] = sees >> i & 1 ? e[i] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[u][i] = (__bf16)e[8 * u + i];
+  }
+};
+
+// A drafted token's value may hold an infinity or a NaN that only some rows see; 0 * inf would hand it to
+// all of them (bf16; an 8-bit code is finite).  The loop takes such values of new tokens out of the
+// product (spare_fresh) and remembers that there were any; behind the loop they are added to the rows
+// that see them: +inf, -inf, or both for a NaN, where a product of indicators counts any.
+__device__ __forceinline__ u32x4 spare_fresh(u32x4 f, uint32_t fresh, bool* spared) {  // 8 slots of one dim
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = f[i];
+    const bool lo = (w & 0x7f80u) == 0x7f80u && (fresh >> (2 * i) & 1);
+    const bool hi = (w & 0x7f800000u) == 0x7f800000u && (fresh >> (2 * i + 1) & 1);
+    f[i] = w & ((lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u));
+    *spared |= lo || hi;
+  }
+  return f;
+}
+template <int D>
+__device__ __forceinline__ void add_specials(const AttnKvArgs& a, int b, const RowLen& len, const bf16_t* v, int tile, int n,
+                                             int h, const Row& row, f32x16* o) {
+  uint32_t live, sees;
+  edge_bits(a, b, len, tile, h, row, &live, &sees);
+  // pairs of 1.0 and 0.0 in bf16
+  auto ones = [](bool lo, bool hi) { return (lo ? 0x3f80u : 0u) | (hi ? 0x3f800000u : 0u); };
+  uint4 one[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const uint32_t m = (sees & (live8(a, b, len, tile * 32 + 16 * u + 8 * h).fresh << (8 * u))) >> (8 * u);
+    one[u] = make_uint4(ones(m & 1, m & 2), ones(m & 4, m & 8), ones(m & 16, m & 32), ones(m & 64, m & 128));
+  }
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t) {
+    uint4 f[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      f[u] = *reinterpret_cast<const uint4*>(v + (size_t)(32 * t + n) * a.c.slots + (size_t)tile * 32 + 16 * u + 8 * h);
+    for (int sg = 0; sg < 2; ++sg) {
+      const uint32_t inf = sg ? 0xff80u : 0x7f80u;
+      auto bad = [&](uint32_t z) { return (z & 0x7fffu) > 0x7f80u || z == inf; };
+      auto pair = [&](uint32_t w) { return ones(bad(w & 0xffffu), bad(w >> 16)); };
+      f32x16 cnt;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) cnt[i] = 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint4 ind = make_uint4(pair(f[u].x), pair(f[u].y), pair(f[u].z), pair(f[u].w));
+        cnt = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, ind), __builtin_bit_cast(bf16x8, one[u]), cnt,
+                                                      0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (cnt[i] > 0.f) o[t][i] += sg ? -INFINITY : INFINITY;
+    }
+  }
+}
+
+// The block's place.  Blocks are dealt round-robin over the 8 XCDs, and over the CUs of each: the row
+// blocks of a unit stay on one XCD, where the second finds the first's keys in L2.  Rows that are split
+// (all blocks are on the card at once) go row block by row block, so that a CU gets different ones (with
+// the row block innermost, CUs got two full ones or two that were nearly empty); unsplit ones, of which
+// there may be many more, go unit by unit.
+struct Place {
+  int unit, rb, hkv, x;
+};
+__device__ __forceinline__ Place place_of(int NS, int least, int RB, int Hkv) {
+  Place p;
+  const int k = (int)(blockIdx.x >> 3), xcd = (int)(blockIdx.x & 7);
+  if (RB == 1) {
+    p.unit = k * 8 + xcd;
+    p.rb = 0;
+  } else if (least) {
+    const int upx = (NS * Hkv + 7) >> 3;
+    p.rb = k / upx;
+    p.unit = (k - p.rb * upx) * 8 + xcd;
+  } else {
+    p.unit = k / RB * 8 + xcd;
+    p.rb = k % RB;
+  }
+  p.hkv = p.unit % Hkv;
+  p.x = p.unit / Hkv;
+  return p;
+}
+
+// Everything that a loop takes from before it has arrived.  (Without it the compiler, which cannot tell the
+// first turn from the others, waits for q's loads in every turn, and with them for the tiles in flight.)
+__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
+
+// this lane's row r: token, tree word, and the q fragments (16-byte pieces of dims 32 j + 16 h + 8 e)
+template <int D>
+__device__ __forceinline__ Row load_row(const AttnKvArgs& a, int b, int hkv, const RowLen& len, int r, int R, int h,
+                                        bf16x8* qf) {
+  const int G = a.Hq / a.c.n_kv;
+  const bool on = r < R;
+  const int t = on ? r / G : 0, g = on ? r - t * G : 0;
+  const bf16_t* q = a.q + ((size_t)b * a.T + t) * a.ldq + (size_t)(hkv * G + g) * D + h * 16;
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      qf[2 * j + e] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(q + 32 * j + 8 * e));
+  const int seen = len.nk - len.start;  // new tokens that have a slot
+  return {t, a.tree ? a.tree[(size_t)b * a.T + t] & (seen >= 64 ? ~0ull : (1ull << seen) - 1) : 0};
+}
+
+// The loads of a tile that W waves share, and their way into LDS as the fragments of the two products
+// (lane l's 16 bytes of fragment k: at k / 2 .. see FB).  8-bit: a wave-wide load is a KiB as it lies, two
+// fragments in bf16.  bf16: 16 rows (K) or dims (V^T) of 64 bytes each, so that a load touches 16 lines
+// and not 64.
+constexpr int FB = 512 + 32;  // bytes of 32 lanes' fragments; 32 more, so that neighbours' writes meet no bank twice
+template <int KT, int D, int W>
+struct Stage {
+  static constexpr bool Q8 = KT != KV_BF16;
+  static constexpr int NG = Q8 ? D / 32 : D / 16;  // wave-wide loads of a tile's K, and of its V
+  static constexpr int NL = (NG + W - 1) / W;
+  static constexpr int BYTES = D / 8 * FB;         // of K, and of V, in LDS
+  u32x4 f[NL];
+  float ks, vs;  // of this lane's slot
+
+  __device__ __forceinline__ void load_scales(const AttnKvArgs& a, size_t head, int tile, int lane) {
+    if constexpr (Q8) {
+      const uint32_t sl = 16 * ((lane & 15) >> 3) + 8 * (lane >> 5) + (lane & 7);
+      ks = (a.c.ks + head + tile * 32)[sl];
+      vs = (a.c.vs + head + tile * 32)[sl];
+    }
+  }
+  // (wave-wide bases and 32 bits of offset a lane: slots is below 2^25)
+  __device__ __forceinline__ void load_k(const char* kb, int tile, int w, int lane) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int g = w + i * W;
+      if (NG % W && g >= NG) break;
+      const char* p = kb + (Q8 ? (size_t)tile * (32 * D) + g * 1024
+                               : ((size_t)tile * 32 + (g & 1) * 16) * (2 * D) + (g >> 1) * 64);
+      f[i] = *reinterpret_cast<const u32x4*>(p + (uint32_t)(Q8 ? lane * 16 : (lane >> 2) * (2 * D) + (lane & 3) * 16));
+    }
+  }
+  __device__ __forceinline__ void load_v(const char* vb, int slots, int tile, int w, int lane) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int g = w + i * W;
+      if (NG % W && g >= NG) break;
+      const char* p = vb + (Q8 ? (size_t)tile * (32 * D) + g * 1024 : ((size_t)(g * 16) * slots + (size_t)tile * 32) * 2);
+      f[i] = *reinterpret_cast<const u32x4*>(p + (uint32_t)(Q8 ? lane * 16 : (lane >> 2) * (2 * slots) + (lane & 3) * 16));
+    }
+  }
+  __device__ __forceinline__ void store_k(int w, int lane, char* kd) {
+    const int n = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int g = w + i * W;
+      if (NG % W && g >= NG) break;
+      if constexpr (Q8) {  // steps 2 g and 2 g + 1
+        put8(kd + (4 * g + h) * FB + n * 16, f[i]);
+      } else {
+        const int cc = (g >> 1) * 4 + (lane & 3);  // the row's 16-byte piece: dims 8 cc..
+        const int m = kv_row_of_slot((g & 1) * 16 + (lane >> 2));
+        *reinterpret_cast<u32x4*>(kd + (((cc >> 2) * 2 + (cc & 1)) * 2 + (cc >> 1 & 1)) * FB + m * 16) = f[i];
+      }
+    }
+  }
+  // true: a new token's value was not finite and has been spared (bf16)
+  __device__ __forceinline__ bool store_v(const AttnKvArgs& a, int b, const RowLen& len, int tile, int w, int lane, char* vd) {
+    const int n = lane & 31, h = lane >> 5;
+    bool spared = false;
+    if (a.mask != nullptr || tile * 32 + 32 > len.start) {
+      if constexpr (Q8) {
+        const uint32_t live = live8(a, b, len, tile * 32 + 8 * h).live | live8(a, b, len, tile * 32 + 16 + 8 * h).live << 8;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) f[i] = clear_dead<KT>(f[i], live);
+      } else {
+        const Live8 l = live8(a, b, len, tile * 32 + (lane & 3) * 8);
+#pragma unroll
+        for (int i = 0; i < NL; ++i) f[i] = spare_fresh(clear_dead<KT>(f[i], l.live), l.fresh, &spared);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int g = w + i * W;
+      if (NG % W && g >= NG) break;
+      if constexpr (Q8) {  // the two halves of the slots
+        put8(vd + (4 * g + h) * FB + n * 16, f[i]);
+      } else {
+        const int d = g * 16 + (lane >> 2);
+        *reinterpret_cast<u32x4*>(vd + ((d >> 5) * 4 + (lane & 3)) * FB + (d & 31) * 16) = f[i];
+      }
+    }
+    return spared;
+  }
+  static __device__ __forceinline__ void put8(char* d, const u32x4& f) {
+    *reinterpret_cast<bf16x8*>(d) = frag8<KT>(f[0], f[1]);
+    *reinterpret_cast<bf16x8*>(d + 2 * FB) = frag8<KT>(f[2], f[3]);
+  }
+};
+
+// Up to 32 rows a KV head (a decode step, a small tree): bound by the cache's bytes.  The NW waves of a
+// block take tiles in turn, loaded one tile ahead, with no barrier in the loop, and merge once at the
+// end.  8-bit fragments go from memory straight into registers, bf16 ones through LDS of the wave's own.
+template <int KT, int D, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void attn_kv_keys(AttnKvArgs a, int NS, int least) {
   constexpr bool Q8 = KT != KV_BF16;
-  constexpr int NF = Q8 ? D / 32 : D / 16;  // 16-byte fragments of K, and of V, a lane takes of a tile
-  constexpr int DT = D / 32;                // 32-dim tiles of the output
-  constexpr int OW = DT > 1 ? 64 : 32;      // dims that one round of the merge holds
-  __shared__ __attribute__((aligned(16))) float os[4][32][OW + 4];
-  __shared__ float mls[4][32 * RT][2];
+  constexpr int NF = D / 32;
+  constexpr int DT = D / 32;
+  using St = Stage<KT, D, 1>;
+  constexpr int OS = 32 * (D + 4) * 4, WL = Q8 || 2 * St::BYTES < OS ? OS : 2 * St::BYTES;  // LDS of a wave
+  __shared__ __attribute__((aligned(16))) char lds[NW * WL];
+  __shared__ float mls[NW][32][2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, h = lane >> 5;
   const int Hkv = a.c.n_kv, G = a.Hq / Hkv, slots = a.c.slots;
-  // blocks are dealt round-robin over the 8 XCDs: the row blocks of one split stay on one, where the
-  // second finds the first's keys in L2
-  const int unit = (int)(blockIdx.x >> 3) / RB * 8 + (blockIdx.x & 7), rb = (blockIdx.x >> 3) % RB;
-  if (unit >= NS * Hkv) return;
-  const int hkv = unit % Hkv, x = unit / Hkv;
-  const Split sp = find_split(a, NS, x, 0);
-  if (sp.b < 0) return;
-  const int b = sp.b;
-  const RowLen len = row_len(a, b);
-  const int R = len.n * G, r0 = rb * 32 * RT;  // rows of this (row, KV head); this block's first
-  if (r0 >= R) return;
-  // a chain's row block sees no slot behind its last token's
-  int nk = len.nk;
-  if (!a.tree) nk = min(nk, len.start + (min(R, r0 + 32 * RT) - 1) / G + 1);
-  const int nt = (nk + 31) >> 5;
-  const int t0 = (int)((int64_t)nt * sp.s / sp.ns), t1 = (int)((int64_t)nt * (sp.s + 1) / sp.ns);
-
-  // ---- this lane's rows: q fragments and what the token sees ----
-  bf16x8 qf[RT][D / 16];
-  uint64_t tw[RT];
-  int tok[RT];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int r = r0 + rt * 32 + n, t = r / G, g = r - t * G;
-    const bool on = r < R;
-    tok[rt] = on ? t : 0;
-    const bf16_t* q = a.q + ((size_t)b * a.T + tok[rt]) * a.ldq + (size_t)(hkv * G + (on ? g : 0)) * D + h * 16;
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        qf[rt][2 * j + e] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(q + 32 * j + 8 * e));
-    const int seen = len.nk - len.start;  // new tokens that have a slot
-    tw[rt] = a.tree ? a.tree[(size_t)b * a.T + tok[rt]] & (seen >= 64 ? ~0ull : (1ull << seen) - 1) : 0;
-  }
-
-  const size_t head = ((size_t)b * Hkv + hkv) * slots;
-  const char* kb = (const char*)a.c.k + head * D * (Q8 ? 1 : 2);
-  const char* vb = (const char*)a.c.v + head * D * (Q8 ? 1 : 2);
-  const int kap = kv_slot_of_row(n);
-  auto load_k = [&](int tile, uint4* f) {
-    if constexpr (Q8) {
-      const char* p = kb + (size_t)tile * (32 * D) + lane * 16;
-#pragma unroll
-      for (int j = 0; j < NF; ++j) f[j] = *reinterpret_cast<const uint4*>(p + j * 1024);
-    } else {
-      const char* p = kb + ((size_t)tile * 32 + kap) * (2 * D) + h * 32;
-#pragma unroll
-      for (int j = 0; j < NF; ++j) f[j] = *reinterpret_cast<const uint4*>(p + (j >> 1) * 64 + (j & 1) * 16);
-    }
-  };
-  auto load_v = [&](int tile, uint4* f) {
-    if constexpr (Q8) {
-      const char* p = vb + (size_t)tile * (32 * D) + lane * 16;
-#pragma unroll
-      for (int j = 0; j < NF; ++j) f[j] = *reinterpret_cast<const uint4*>(p + j * 1024);
-    } else {
-      const char* p = vb + ((size_t)n * slots + (size_t)tile * 32 + 8 * h) * 2;
-#pragma unroll
-      for (int j = 0; j < NF; ++j) f[j] = *reinterpret_cast<const uint4*>(p + (size_t)(j >> 1) * 64 * slots + (j & 1) * 32);
-    }
-  };
-  auto k_frag = [&](const uint4* f, int s) -> bf16x8 {  // step s of the 16-dim steps
-    if constexpr (Q8) return s & 1 ? frag8<KT>(f[s >> 1].z, f[s >> 1].w) : frag8<KT>(f[s >> 1].x, f[s >> 1].y);
-    else return __builtin_bit_cast(bf16x8, f[s]);
-  };
-  auto v_frag = [&](const uint4* f, int t, int u) -> bf16x8 {
-    if constexpr (Q8) return u ? frag8<KT>(f[t].z, f[t].w) : frag8<KT>(f[t].x, f[t].y);
-    else return __builtin_bit_cast(bf16x8, f[2 * t + u]);
-  };
-
-  f32x16 o[RT][DT];
-  float m[RT], l[RT];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    m[rt] = -INFINITY;
-    l[rt] = 0.f;
-#pragma unroll
-    for (int t = 0; t < DT; ++t)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[rt][t][i] = 0.f;
-  }
+  const Place pl = place_of(NS, least, 1, Hkv);
+  if (pl.unit >= NS * Hkv) return;
   const float c = a.scale * 1.44269504088896340736f;  // softmax in powers of two
+  const uint32_t sl = 16 * ((lane & 15) >> 3) + 8 * h + (lane & 7);  // the slot whose scales this lane holds
+  char* mylds = lds + wave * WL;
 
-  uint4 kf[NF], vf[NF];
-  int tile = t0 + wave;
-  if (tile < t1) {
-    load_k(tile, kf);
-    load_v(tile, vf);
-  }
-  for (; tile < t1; tile += 4) {
-    const int nxt = min(tile + 4, t1 - 1);  // (the last turn reads its own tile again: in bounds)
-    f32x16 s[RT];
+  for_segments(a, NS, least, pl.x, blockIdx.x == 0, [&](const Seg& sg) {
+    const int b = sg.b;
+    const RowLen len = sg.len;
+    const int R = len.n * G;
+    if (R == 0) return;
+    const int t1 = min(sg.t1, (len.nk + 31) >> 5);
+    int tile = sg.t0 + wave;
+    const size_t head = ((size_t)b * Hkv + pl.hkv) * slots;
+    const char* kb = (const char*)a.c.k + head * D * (Q8 ? 1 : 2);
+    const char* vb = (const char*)a.c.v + head * D * (Q8 ? 1 : 2);
+    u32x4 kf[NF], vf[NF];  // 8-bit
+    St sk, sv;             // bf16
+    float ksn = 0.f, vsn = 0.f;
+    auto load_k = [&](int t) {
+      const char* p = kb + (size_t)t * (32 * D);
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
+      for (int j = 0; j < NF; ++j) kf[j] = *reinterpret_cast<const u32x4*>(p + (uint32_t)(j * 1024 + lane * 16));
+      ksn = (a.c.ks + head + t * 32)[sl];
+      vsn = (a.c.vs + head + t * 32)[sl];
+    };
+    auto load_v = [&](int t) {
+      const char* p = vb + (size_t)t * (32 * D);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[rt][i] = 0.f;
-#pragma unroll
-    for (int j = 0; j < D / 16; ++j) {
-      const bf16x8 k = k_frag(kf, j);
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) s[rt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, qf[rt][j], s[rt], 0, 0, 0);
-    }
-    load_k(nxt, kf);
-    float vs[16];
-    if constexpr (Q8) {
-      float ks[16];
-      const float* p = a.c.ks + head + tile * 32 + 8 * h;
-      const float* w = a.c.vs + head + tile * 32 + 8 * h;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int i = 0; i < 8; i += 4) {
-          *reinterpret_cast<float4*>(&ks[8 * u + i]) = *reinterpret_cast<const float4*>(p + 16 * u + i);
-          *reinterpret_cast<float4*>(&vs[8 * u + i]) = *reinterpret_cast<const float4*>(w + 16 * u + i);
-        }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float kc = ks[i] * c;
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) s[rt][i] *= kc;
+      for (int j = 0; j < NF; ++j) vf[j] = *reinterpret_cast<const u32x4*>(p + (uint32_t)(j * 1024 + lane * 16));
+    };
+    if (tile < t1) {
+      if constexpr (Q8) {
+        load_k(tile);
+        load_v(tile);
+      } else {
+        sk.load_k(kb, tile, 0, lane);
+        sv.load_v(vb, slots, tile, 0, lane);
       }
-    } else {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[rt][i] *= c;
     }
-    uint32_t sees[RT];  // bit 8 u + i: the row sees slot 16 u + 8 h + i of the tile
-    const bool edge = a.mask != nullptr || tile * 32 + 32 > len.start;
-    if (edge) {
-      uint32_t live = 0;  // slots that some row may see: the others' bytes are anything
+    bf16x8 qf[D / 16];
+    const Row row = load_row<D>(a, b, pl.hkv, len, n, R, h, qf);
+    RowState<KT, D> st;
+    st.clear();
+    bool spared = false;
+    loads_done();
+    for (; tile < t1; tile += NW) {
+      const int nxt = min(tile + NW, t1 - 1);  // (the last turn reads its own tile or a later one again: in bounds)
+      f32x16 s;
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) sees[rt] = 0;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int k0 = tile * 32 + 16 * u + 8 * h, d0 = k0 - len.start;  // d0: the first slot's new token
-        const int cn = min(max(-d0, 0), 8), ln = min(max(len.nk - k0, 0), 8);
-        uint32_t ctx = (1u << cn) - 1;
-        const uint32_t fresh = ((1u << ln) - 1) & ~ctx;
-        if (a.mask) {
-          const uint2 mk = *reinterpret_cast<const uint2*>(a.mask + (size_t)b * slots + k0);
-          uint32_t mb = 0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            mb |= ((mk.x >> (8 * i)) & 0xff ? 1u << i : 0) | ((mk.y >> (8 * i)) & 0xff ? 16u << i : 0);
-          ctx &= mb;
-        }
-        live |= (ctx | fresh) << (8 * u);
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          uint32_t w;
-          if (a.tree) w = d0 >= 0 ? (d0 < 64 ? (uint32_t)(tw[rt] >> d0) : 0) : d0 > -8 ? (uint32_t)tw[rt] << -d0 : 0;
-          else w = (1u << min(max(tok[rt] + 1 - d0, 0), 8)) - 1;
-          sees[rt] |= (ctx | (fresh & w)) << (8 * u);
-        }
-      }
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[rt][i] = sees[rt] >> i & 1 ? s[rt][i] : -INFINITY;
-      // values of slots that nobody sees (never written, padded away) must not reach a product
+      for (int i = 0; i < 16; ++i) s[i] = 0.f;
+      const char* kp = mylds + h * FB + n * 16;
       if constexpr (Q8) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t keep = 0;
-#pragma unroll
-          for (int y = 0; y < 4; ++y) keep |= live >> (4 * w + y) & 1 ? 0xffu << (8 * y) : 0;
-#pragma unroll
-          for (int j = 0; j < NF; ++j) {
-            uint32_t& z = reinterpret_cast<uint32_t*>(&vf[j])[w];
-            z &= keep;
-            if constexpr (KT == KV_E4M3) {
-              // (append writes no NaN code, a NaN row has a NaN scale; a new token's slot that was never
-              // written may hold one, and rows that do not see it are spared)
-              const uint32_t nan = (((z & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
-              z &= ~(nan * 0xffu);
-            }
-          }
+        for (int j = 0; j < D / 16; ++j) {
+          const bf16x8 k = j & 1 ? frag8<KT>(kf[j >> 1].z, kf[j >> 1].w) : frag8<KT>(kf[j >> 1].x, kf[j >> 1].y);
+          s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, qf[j], s, 0, 0, 0);
         }
       } else {
+        sk.store_k(0, lane, mylds);
+        spared |= sv.store_v(a, b, len, tile, 0, lane, mylds + St::BYTES);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        sk.load_k(kb, nxt, 0, lane);
+        sv.load_v(vb, slots, nxt, 0, lane);
+        bf16x8 k[D / 16];
 #pragma unroll
-        for (int w = 0; w < 8; ++w) {
-          const uint32_t keep = (live >> (2 * w) & 1 ? 0xffffu : 0) | (live >> (2 * w + 1) & 1 ? 0xffff0000u : 0);
+        for (int j = 0; j < D / 16; ++j) k[j] = *reinterpret_cast<const bf16x8*>(kp + 2 * j * FB);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int t = 0; t < DT; ++t) reinterpret_cast<uint32_t*>(&vf[2 * t + (w >> 2)])[w & 3] &= keep;
-        }
+        for (int j = 0; j < D / 16; ++j) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[j], qf[j], s, 0, 0, 0);
       }
-    }
-    bf16x8 p[RT][2];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      float mx = s[rt][0];
-#pragma unroll
-      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[rt][i]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      if (__any(mx > m[rt])) {
-        const float mn = fmaxf(m[rt], mx);
-        const float al = m[rt] == -INFINITY ? (mn == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(m[rt] - mn);
-        m[rt] = mn;
-        l[rt] *= al;
-#pragma unroll
-        for (int t = 0; t < DT; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[rt][t][i] *= al;
-      }
-      const float mu = m[rt] == -INFINITY ? 0.f : m[rt];
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float e = __builtin_amdgcn_exp2f(s[rt][8 * u + i] - mu);
-          l[rt] += e;
-          float w = e;
-          // (a slot's scale counts for the rows that see it alone)
-          if constexpr (Q8) w = edge && !(sees[rt] >> (8 * u + i) & 1) ? 0.f : e * vs[8 * u + i];
-          // p is rounded to bf16, the product's type: half a step of 2^-8 at random signs over the
-          // keys, less than the output's own rounding
-          p[rt][u][i] = (__bf16)w;
-        }
-    }
-    if constexpr (!Q8) {
-      // A drafted token's value may hold an infinity or a NaN that only some rows see; 0 * inf would
-      // hand it to all of them.  Such values are taken out of the product and added to the rows that
-      // see them: as many +inf (NaN: both signs) as there are, found by a product of indicators.
-      bool bad = false;
+      const float kcl = ksn * c;
+      float vsl = vsn;
+      if constexpr (Q8) load_k(nxt);
+      const bool edge = a.mask != nullptr || tile * 32 + 32 > len.start;
+      bool special = false;
+      uint32_t live = 0xffff, sees = 0xffff;
       if (edge) {
+        edge_bits(a, b, len, tile, h, row, &live, &sees);
+        if constexpr (Q8) {
 #pragma unroll
-        for (int j = 0; j < NF; ++j)
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const uint32_t z = reinterpret_cast<uint32_t*>(&vf[j])[w];
-            bad |= (z & 0x7f80u) == 0x7f80u || (z & 0x7f800000u) == 0x7f800000u;
-          }
+          for (int j = 0; j < NF; ++j) vf[j] = clear_dead<KT>(vf[j], live);
+          vsl = live >> (lane & 15) & 1 ? vsl : 0.f;
+          special = __any(!(fabsf(vsl) < INFINITY));
+        }
       }
-      if (__any(bad)) {
+      bf16x8 p[2];
+      st.scores(s, c, kcl, edge, sees);
+      st.probs(s, c, vsl, sees, special, p);
 #pragma unroll
-        for (int t = 0; t < DT; ++t) {
+      for (int t = 0; t < DT; ++t)
 #pragma unroll
-          for (int sg = 0; sg < 2; ++sg) {
-            bf16x8 ind[2];
+        for (int u = 0; u < 2; ++u) {
+          bf16x8 v;
+          if constexpr (Q8) v = u ? frag8<KT>(vf[t].z, vf[t].w) : frag8<KT>(vf[t].x, vf[t].y);
+          else v = *reinterpret_cast<const bf16x8*>(kp + St::BYTES + (4 * t + 2 * u) * FB);
+          st.o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, p[u], st.o[t], 0, 0, 0);
+        }
+      if constexpr (Q8) load_v(nxt);
+      else __builtin_amdgcn_wave_barrier();
+    }
+    if constexpr (!Q8)
+      if (__any(spared))
+        for (tile = sg.t0 + wave; tile < t1; tile += NW)
+          if (tile * 32 + 32 > len.start) add_specials<D>(a, b, len, (const bf16_t*)vb, tile, n, h, row, st.o);
+
+    // ---- the block's waves into one (m, l, o), in wave order ----
+    st.l = half_sum(st.l);
+    if (h == 0) {
+      mls[wave][n][0] = st.m;
+      mls[wave][n][1] = st.l;
+    }
+    __syncthreads();
+    float M = -INFINITY, L = 0.f, mine = 0.f;
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, mls[w][n][0]);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const uint32_t z = reinterpret_cast<const uint32_t*>(&vf[2 * t + u])[i >> 1] >> (16 * (i & 1)) & 0xffff;
-                const bool nan = (z & 0x7fff) > 0x7f80, inf = z == (sg ? 0xff80u : 0x7f80u);
-                ind[u][i] = nan || inf ? (__bf16)1.0f : (__bf16)0.0f;
-              }
+    for (int w = 0; w < NW; ++w) {
+      const float mw = mls[w][n][0];
+      const float f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - M);
+      L += mls[w][n][1] * f;
+      if (w == wave) mine = f;
+    }
+    // (a row that saw nothing is 0; a whole row is divided here, a split one by the join)
+    const bool whole = sg.slot < 0;
+    const float sc = !whole ? mine : L == 0.f ? 0.f : mine / L;
+    float* po = a.part + head_floats(a.B) + (size_t)(sg.slot * Hkv + pl.hkv) * 32 * (D + 2);
+    if (!whole && wave == 0 && h == 0) *reinterpret_cast<float2*>(po + 32 * D + n * 2) = make_float2(M, L);
+    float* os = reinterpret_cast<float*>(mylds) + n * (D + 4) + 4 * h;
+    if (n < R) {
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-              f32x16 cnt;
+      for (int t = 0; t < DT; ++t)
 #pragma unroll
-              for (int i = 0; i < 16; ++i) cnt[i] = 0.f;
+        for (int i = 0; i < 16; i += 4)
+          *reinterpret_cast<float4*>(os + 32 * t + 2 * i) =
+              make_float4(st.o[t][i] * sc, st.o[t][i + 1] * sc, st.o[t][i + 2] * sc, st.o[t][i + 3] * sc);
+    }
+    __syncthreads();
+    for (int q = threadIdx.x; q < R * (D / 4); q += 64 * NW) {
+      const int r = q / (D / 4), d = q % (D / 4) * 4;
+      const char* src = lds + (r * (D + 4) + d) * 4;
+      float4 y = *reinterpret_cast<const float4*>(src);
 #pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                bf16x8 one;
+      for (int w = 1; w < NW; ++w) {
+        const float4 z = *reinterpret_cast<const float4*>(src + w * WL);
+        y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
+      }
+      if (!whole) {
+        *reinterpret_cast<float4*>(po + r * D + d) = y;
+      } else {
+        const int tk = r / G;
+        bf16_t* dst = a.out + ((size_t)b * a.T + tk) * a.ldo + (size_t)(pl.hkv * G + r - tk * G) * D + d;
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(y.x, y.y), pack2(y.z, y.w));
+      }
+    }
+    if (least) __syncthreads();  // (the next segment writes LDS)
+  });
+}
+
+// More rows: bound by the arithmetic on the scores.  The W waves of a block, 32 rows each, go through the
+// same tiles, whose fragments they load, turn into bf16 and put into LDS together, once for all rows, one
+// tile ahead of the products (two LDS buffers, one barrier a tile).
+template <int KT, int D, int W>
+__global__ __launch_bounds__(64 * W, 2) void attn_kv_rows(AttnKvArgs a, int NS,
+                                                                                              int least, int RB) {
+  constexpr bool Q8 = KT != KV_BF16;
+  constexpr int DT = D / 32, rows = 32 * W;
+  constexpr int TT = W == 2 ? 1 : 2;  // tiles a turn (LDS for 4 blocks of 2 waves, or 2 of 4, or 1 of 8)
+  using St = Stage<KT, D, W>;
+  __shared__ __attribute__((aligned(16))) char lk[2][TT][St::BYTES], lv[2][TT][St::BYTES];
+  __shared__ int spared;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 31, h = lane >> 5;
+  const int Hkv = a.c.n_kv, G = a.Hq / Hkv, slots = a.c.slots;
+  const Place pl = place_of(NS, least, RB, Hkv);
+  if (pl.unit >= NS * Hkv) return;
+  const float c = a.scale * 1.44269504088896340736f;
+
+  for_segments(a, NS, least, pl.x, blockIdx.x == 0, [&](const Seg& sg) {
+    const int b = sg.b;
+    const RowLen len = sg.len;
+    const int r0 = pl.rb * rows, Rend = min(len.n * G, r0 + rows);  // this block's rows of (row, KV head)
+    if (r0 >= Rend) return;
+    // a chain's row block sees no slot behind its last token's
+    const int nk = a.tree ? len.nk : min(len.nk, len.start + (Rend - 1) / G + 1);
+    const int t0 = sg.t0, t1 = min(sg.t1, (nk + 31) >> 5);
+    const int myr = r0 + wave * 32 + n;
+    const bool act = r0 + wave * 32 < Rend;  // (a wave without rows only helps with the tiles)
+
+    const size_t head = ((size_t)b * Hkv + pl.hkv) * slots;
+    const char* kb = (const char*)a.c.k + head * D * (Q8 ? 1 : 2);
+    const char* vb = (const char*)a.c.v + head * D * (Q8 ? 1 : 2);
+    RowState<KT, D> st;
+    st.clear();
+    if (threadIdx.x == 0) spared = 0;
+    // A turn works on TT tiles out of one half of LDS, while the next TT go from registers into the other
+    // half and the TT behind them are loaded: what a turn waits for was asked for a whole turn ago.
+    St gk[TT], gv[TT];
+    float ks[TT], vs[TT], kn[TT], vn[TT];  // scales of this turn's tiles and of the next one's
+    const uint32_t at = h * FB + n * 16;
+    auto fetch = [&](int tile) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) one[i] = sees[rt] >> (8 * u + i) & 1 ? (__bf16)1.0f : (__bf16)0.0f;
-                cnt = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ind[u], one, cnt, 0, 0, 0);
-              }
+      for (int i = 0; i < TT; ++i) {
+        const int t = min(tile + i, t1 - 1);  // (past the end the last tile again: in bounds, not used)
+        gk[i].load_scales(a, head, t, lane);
+        gk[i].load_k(kb, t, wave, lane);
+        gv[i].load_v(vb, slots, t, wave, lane);
+      }
+    };
+    auto put = [&](int tile, int half) {
 #pragma unroll
-              for (int i = 0; i < 16; ++i)
-                if (cnt[i] > 0.f) o[rt][t][i] += sg ? -INFINITY : INFINITY;
+      for (int i = 0; i < TT; ++i) {
+        gk[i].store_k(wave, lane, lk[half][i]);
+        if (gv[i].store_v(a, b, len, min(tile + i, t1 - 1), wave, lane, lv[half][i])) spared = 1;
+        if constexpr (Q8) {
+          kn[i] = gk[i].ks * c;
+          vn[i] = gk[i].vs;
+        }
+      }
+    };
+    if (t0 < t1) fetch(t0);
+    bf16x8 qf[D / 16];
+    const Row row = load_row<D>(a, b, pl.hkv, len, myr, Rend, h, qf);
+    __syncthreads();  // (spared is 0, and the last segment's tiles have been read)
+    loads_done();
+    if (t0 < t1) {
+      put(t0, 0);
+      fetch(t0 + TT);
+    }
+    for (int tile = t0, half = 0; tile < t1; tile += TT, half ^= 1) {
+      if constexpr (Q8) {
+#pragma unroll
+        for (int i = 0; i < TT; ++i) {
+          ks[i] = kn[i];
+          vs[i] = vn[i];
+        }
+      }
+      __syncthreads();  // this turn's fragments are there, the other half has been read
+      if (tile + TT < t1) {
+        put(tile + TT, half ^ 1);
+        fetch(tile + 2 * TT);
+      }
+      if (act) {
+#pragma unroll
+        for (int i = 0; i < TT; ++i) {
+          const int tl = tile + i;
+          if (tl >= t1) break;
+          const char *kp = lk[half][i] + at, *vp = lv[half][i] + at;
+          // (all reads before the first product: one at a time, each product waits out LDS's latency)
+          bf16x8 k[D / 16];
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j) k[j] = *reinterpret_cast<const bf16x8*>(kp + 2 * j * FB);
+          __builtin_amdgcn_sched_barrier(0);
+          f32x16 s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[0], qf[0], f32x16{}, 0, 0, 0);
+#pragma unroll
+          for (int j = 1; j < D / 16; ++j) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[j], qf[j], s, 0, 0, 0);
+          const bool edge = a.mask != nullptr || tl * 32 + 32 > len.start;
+          bool special = false;
+          uint32_t live = 0xffff, sees = 0xffff;
+          float vsl = vs[i];
+          if (edge) {
+            edge_bits(a, b, len, tl, h, row, &live, &sees);
+            if constexpr (Q8) {
+              vsl = live >> (lane & 15) & 1 ? vsl : 0.f;
+              special = __any(!(fabsf(vsl) < INFINITY));
             }
           }
+          st.scores(s, c, ks[i], edge, sees);
+          bf16x8 p[2];
+          st.probs(s, c, vsl, sees, special, p);
+          bf16x8 v[DT][2];
+#pragma unroll
+          for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) v[t][u] = *reinterpret_cast<const bf16x8*>(vp + (4 * t + 2 * u) * FB);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              uint32_t& z = reinterpret_cast<uint32_t*>(&vf[2 * t + u])[w];
-              if ((z & 0x7f80u) == 0x7f80u) z &= 0xffff0000u;
-              if ((z & 0x7f800000u) == 0x7f800000u) z &= 0xffffu;
-            }
+            for (int t = 0; t < DT; ++t)
+              st.o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[t][u], p[u], st.o[t], 0, 0, 0);
         }
       }
     }
-#pragma unroll
-    for (int t = 0; t < DT; ++t)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const bf16x8 v = v_frag(vf, t, u);
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) o[rt][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, p[rt][u], o[rt][t], 0, 0, 0);
-      }
-    load_v(nxt, vf);
-  }
-
-  // ---- the block's 4 waves into one (m, l, o), in wave order ----
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    l[rt] += __shfl_xor(l[rt], 32, 64);
-    if (h == 0) {
-      mls[wave][rt * 32 + n][0] = m[rt];
-      mls[wave][rt * 32 + n][1] = l[rt];
-    }
-  }
-  __syncthreads();
-  float* po = a.part + ((size_t)((size_t)x * Hkv + hkv) * RB + rb) * (32 * RT) * (D + 2);
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    float M = -INFINITY, L = 0.f, f[4];
-#pragma unroll
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, mls[w][rt * 32 + n][0]);
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float mw = mls[w][rt * 32 + n][0];
-      f[w] = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - M);
-      L += mls[w][rt * 32 + n][1] * f[w];
-    }
-    const float mine = wave == 0 ? f[0] : wave == 1 ? f[1] : wave == 2 ? f[2] : f[3];
-    // (a row that saw nothing is 0; one block's row is divided here, a split one's by the join)
-    const float sc = sp.ns > 1 ? mine : L == 0.f ? 0.f : mine / L;
-    if (sp.ns > 1 && wave == 0 && h == 0) {
-      po[(size_t)(32 * RT) * D + (rt * 32 + n) * 2] = M;
-      po[(size_t)(32 * RT) * D + (rt * 32 + n) * 2 + 1] = L;
-    }
-#pragma unroll
-    for (int d0 = 0; d0 < D; d0 += OW) {
-#pragma unroll
-      for (int t = 0; t < OW / 32; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const f32x16& v = o[rt][d0 / 32 + t];
-          *reinterpret_cast<float4*>(&os[wave][n][32 * t + 2 * i + 4 * h]) =
-              make_float4(v[i] * sc, v[i + 1] * sc, v[i + 2] * sc, v[i + 3] * sc);
-        }
+    if constexpr (!Q8) {
       __syncthreads();
-#pragma unroll
-      for (int q = threadIdx.x; q < 32 * OW / 4; q += 256) {
-        const int row = q / (OW / 4), d = q % (OW / 4) * 4, r = r0 + rt * 32 + row;
-        float4 y = *reinterpret_cast<const float4*>(&os[0][row][d]);
-#pragma unroll
-        for (int w = 1; w < 4; ++w) {
-          const float4 z = *reinterpret_cast<const float4*>(&os[w][row][d]);
-          y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
-        }
-        if (r < R) {
-          if (sp.ns > 1) {
-            *reinterpret_cast<float4*>(po + (size_t)(rt * 32 + row) * D + d0 + d) = y;
-          } else {
-            const int t = r / G;
-            bf16_t* dst = a.out + ((size_t)b * a.T + t) * a.ldo + (size_t)(hkv * G + r - t * G) * D + d0 + d;
-            *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(y.x, y.y), pack2(y.z, y.w));
-          }
-        }
-      }
-      __syncthreads();
+      if (spared && act)
+        for (int tile = max(t0, len.start >> 5); tile < t1; ++tile)
+          add_specials<D>(a, b, len, (const bf16_t*)vb, tile, n, h, row, st.o);
+      if (least) __syncthreads();  // (the next segment clears it)
     }
-  }
+    st.l = half_sum(st.l);
+    if (myr >= Rend) return;
+    if (sg.slot >= 0) {  // a split row is divided by the join
+      float* po = a.part + head_floats(a.B) + ((size_t)(sg.slot * Hkv + pl.hkv) * RB + pl.rb) * rows * (D + 2);
+      const int rr = wave * 32 + n;
+      if (h == 0) *reinterpret_cast<float2*>(po + (size_t)rows * D + rr * 2) = make_float2(st.m, st.l);
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          *reinterpret_cast<float4*>(po + (size_t)rr * D + 32 * t + 2 * i + 4 * h) =
+              make_float4(st.o[t][i], st.o[t][i + 1], st.o[t][i + 2], st.o[t][i + 3]);
+    } else {
+      const float sc = st.l == 0.f ? 0.f : 1.f / st.l;  // (a row that saw nothing is 0)
+      bf16_t* dst = a.out + ((size_t)b * a.T + row.tok) * a.ldo + (size_t)(pl.hkv * G + myr - row.tok * G) * D;
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          *reinterpret_cast<uint2*>(dst + 32 * t + 2 * i + 4 * h) =
+              make_uint2(pack2(st.o[t][i] * sc, st.o[t][i + 1] * sc), pack2(st.o[t][i + 2] * sc, st.o[t][i + 3] * sc));
+    }
+  });
 }
 
-// Joins the splits of a row: a wave per (token, q head), partials in split order.
-template <int D>
-__global__ __launch_bounds__(256) void attn_kv_join(AttnKvArgs a, int NS, int RB, int rows) {
-  const int lane = threadIdx.x & 63;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (w >= (int64_t)a.B * a.T * a.Hq) return;
-  const int hq = (int)(w % a.Hq), t = (int)(w / a.Hq % a.T), b = (int)(w / a.Hq / a.T);
-  if (t >= row_len(a, b).n) return;
-  const Split sp = find_split(a, NS, -1, b);
-  if (sp.ns == 1) return;
-  const int G = a.Hq / a.c.n_kv, hkv = hq / G, r = t * G + hq % G, rb = r / rows, rr = r % rows;
-  const size_t step = (size_t)a.c.n_kv * RB * rows * (D + 2);  // from one split to the next
-  const float* p = a.part + ((size_t)((size_t)sp.x0 * a.c.n_kv + hkv) * RB + rb) * rows * (D + 2);
+// Joins the partials of a row: GS groups of D / 4 threads (4 dims each) take every GS-th block's partial,
+// four loads in flight, and the groups' sums are added in order.
+template <int D, int GS>
+__global__ __launch_bounds__(256) void attn_kv_join(AttnKvArgs a, int RB, int rows) {
+  constexpr int TR = D / 4, RP = 256 / (TR * GS);  // threads a group, rows a block
+  __shared__ float ms[RP][GS], ls[RP][GS];
+  __shared__ __attribute__((aligned(16))) float ys[RP][GS][D];
+  const int d = threadIdx.x % TR * 4, g = threadIdx.x / TR % GS, row = threadIdx.x / (TR * GS);
+  const int64_t w = (int64_t)blockIdx.x * RP + row;
+  const int TH = a.T * a.Hq, b = (int)min(w / TH, (int64_t)a.B - 1), th = (int)(w - (int64_t)b * TH), t = th / a.Hq,
+            hq = th - t * a.Hq;
+  const int2 xs = *reinterpret_cast<const int2*>(a.part + 2 * b);
+  const int x0 = xs.x, ns = xs.y;
+  const bool on = th < TH && ns > 1 && !(a.counts && t >= a.counts[b]);
   float M = -INFINITY, L = 0.f;
-  for (int s = lane; s < sp.ns; s += 64) M = fmaxf(M, p[s * step + (size_t)rows * D + rr * 2]);
-  M = wave_max(M);
-  constexpr int E = D > 64 ? 2 : 1;  // dims a lane
-  float y[E];
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (on) {
+    const int G = a.Hq / a.c.n_kv, hkv = hq / G, r = t * G + hq - hkv * G, rb = r / rows, rr = r - rb * rows;
+    const size_t step = (size_t)a.c.n_kv * RB * rows * (D + 2);  // from one slot to the next
+    const float* p = a.part + head_floats(a.B) + (size_t)(hkv * RB + rb) * rows * (D + 2);
+    const float *pm = p + (size_t)rows * D + rr * 2, *po = p + (size_t)rr * D + d;
+    // the row begins in block x0 (slot 2 x0 + 1) and goes on in slots 2 x0 + 2, 2 x0 + 4, ..
+    for (int s0 = g; s0 < ns; s0 += 4 * GS) {
+      float2 ml[4];
+      float4 v[4];
 #pragma unroll
-  for (int e = 0; e < E; ++e) y[e] = 0.f;
-  for (int s0 = 0; s0 < sp.ns; s0 += 64) {
-    float f = 0.f;
-    if (s0 + lane < sp.ns) {
-      const float* ml = p + (s0 + lane) * step + (size_t)rows * D + rr * 2;
-      f = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - M);
-      L += f * ml[1];
-    }
-    const int n = min(64, sp.ns - s0);
-#pragma unroll 8
-    for (int s = 0; s < n; ++s) {
-      const float fs = __shfl(f, s, 64);
-      const float* src = p + (s0 + s) * step + (size_t)rr * D + lane * E;
-      if (D >= 64 || lane < D) {
+      for (int i = 0; i < 4; ++i) {
+        const int s = min(s0 + i * GS, ns - 1);
+        const size_t at = (size_t)(2 * x0 + (s ? 2 * s : 1)) * step;
+        ml[i] = *reinterpret_cast<const float2*>(pm + at);
+        v[i] = *reinterpret_cast<const float4*>(po + at);
+      }
+      float mx = M;
 #pragma unroll
-        for (int e = 0; e < E; ++e) y[e] += fs * src[e];
+      for (int i = 0; i < 4; ++i) mx = s0 + i * GS < ns ? fmaxf(mx, ml[i].x) : mx;
+      const float al = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mx);
+      M = mx;
+      L *= al;
+      y.x *= al; y.y *= al; y.z *= al; y.w *= al;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (s0 + i * GS >= ns) break;
+        const float f = ml[i].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[i].x - M);
+        L += f * ml[i].y;
+        y.x += f * v[i].x; y.y += f * v[i].y; y.z += f * v[i].z; y.w += f * v[i].w;
       }
     }
   }
-  L = wave_sum(L);
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  bf16_t* dst = a.out + ((size_t)b * a.T + t) * a.ldo + (size_t)hq * D + lane * E;
-  if constexpr (E == 2) *reinterpret_cast<uint32_t*>(dst) = pack2(y[0] * inv, y[1] * inv);
-  else if (D >= 64 || lane < D) *dst = f2bf(y[0] * inv);
+  if constexpr (GS > 1) {
+    *reinterpret_cast<float4*>(&ys[row][g][d]) = y;
+    if (d == 0) {
+      ms[row][g] = M;
+      ls[row][g] = L;
+    }
+    __syncthreads();
+    if (g) return;
+    float mx = M;
+#pragma unroll
+    for (int i = 1; i < GS; ++i) mx = fmaxf(mx, ms[row][i]);
+    L = 0.f;
+    y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < GS; ++i) {
+      const float m = ms[row][i], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mx);
+      const float4 v = *reinterpret_cast<const float4*>(&ys[row][i][d]);
+      L += f * ls[row][i];
+      y.x += f * v.x; y.y += f * v.y; y.z += f * v.z; y.w += f * v.w;
+    }
+  }
+  if (!on) return;
+  const float inv = L == 0.f ? 0.f : 1.f / L;  // (a row that saw nothing is 0)
+  bf16_t* dst = a.out + ((size_t)b * a.T + t) * a.ldo + (size_t)hq * D + d;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(y.x * inv, y.y * inv), pack2(y.z * inv, y.w * inv));
 }
 
-// The launch: row tiles of 32 a wave (RT), row blocks and splits.  RT 2 halves the loads of a key for
-// trees of more than 32 rows a KV head.
+// The launch: the form (W = 0: attn_kv_keys; else attn_kv_rows of W waves), its row blocks, the blocks NS
+// that share the tiles and the least share (0: a block a row).
 struct AkvPlan {
-  int RT, RB, NS;
+  int W, RB, NS, least;
 };
 static AkvPlan plan(int B, int T, int Hq, int n_kv, int slots, int max_len) {
   AkvPlan p;
-  const int64_t R = (int64_t)T * (Hq / n_kv);
-  p.RT = R > 32 ? 2 : 1;
-  p.RB = (int)((R + 32 * p.RT - 1) / (32 * p.RT));
-  // enough blocks for every CU to hold two (RT 2: one), no split under 4 tiles of the longest row
-  const int64_t want = (p.RT == 1 ? 512 : 256) / std::max<int64_t>(1, (int64_t)n_kv * p.RB);
+  const int64_t R = (int64_t)T * (Hq / n_kv), rt = (R + 31) / 32;
+  p.W = rt <= 1 ? 0 : rt <= 2 ? 2 : rt <= 4 ? 4 : 8;
+  p.RB = p.W ? (int)((rt + p.W - 1) / p.W) : 1;
   const int64_t len = std::min<int64_t>(slots, (int64_t)(max_len > 0 ? std::min(max_len, slots) : slots) + T);
-  const int64_t most = (int64_t)B * std::max<int64_t>(1, ((len + 31) / 32 + 3) / 4);
-  p.NS = (int)std::max<int64_t>(B, std::min(want, most));
+  const int64_t tiles = (len + 31) / 32;                              // of the longest row
+  const int64_t units = std::max<int64_t>(1, (int64_t)n_kv * p.RB);   // blocks a row, unsplit
+  const int64_t room = 256 * (p.W == 0 ? 1 : 8 / p.W);                // blocks that the card holds at once
+  const int64_t most = p.W == 0 ? 32 : 8, least = p.W == 0 ? 8 : 4;
+  p.least = (int)least;
+  p.NS = (int)std::max<int64_t>(1, std::min(room / units, (int64_t)B * ((tiles + least - 1) / least)));
+  // short rows, or enough of them: nothing to join
+  if (tiles <= most || p.NS <= B) {
+    p.least = 0;
+    p.NS = B;
+  }
   return p;
 }
 
 size_t attn_kv_ws_bytes(int B, int T, int Hq, int n_kv, int D, int slots, int max_len) {
   const AkvPlan p = plan(B, T, Hq, n_kv, slots, max_len);
-  if (p.NS <= B) return 0;
-  return (size_t)p.NS * n_kv * p.RB * 32 * p.RT * (D + 2) * sizeof(float);
+  if (p.least == 0) return 0;
+  return (head_floats(B) + (size_t)2 * p.NS * n_kv * p.RB * 32 * std::max(1, p.W) * (D + 2)) * sizeof(float);
 }
 
 template <int KT, int D>
 static hipError_t launch(const AttnKvArgs& a, const AkvPlan& p, hipStream_t s) {
   const int64_t grid = ((int64_t)p.NS * a.c.n_kv + 7) / 8 * 8 * p.RB;
-  if (grid > INT_MAX) return hipErrorInvalidValue;
-  if (p.RT == 1) hipLaunchKernelGGL((attn_kv_kernel<KT, D, 1>), dim3((unsigned)grid), dim3(256), 0, s, a, p.NS, p.RB);
-  else hipLaunchKernelGGL((attn_kv_kernel<KT, D, 2>), dim3((unsigned)grid), dim3(256), 0, s, a, p.NS, p.RB);
-  if (p.NS > a.B) {
-    const int64_t waves = (int64_t)a.B * a.T * a.Hq;
-    if ((waves + 3) / 4 > INT_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(attn_kv_join<D>, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, s, a, p.NS, p.RB, 32 * p.RT);
+  const int GS = p.NS > 4 * a.B ? 8 : 1;  // (rows of many partials: they are read at once, not one after the other)
+  const int64_t join = ((int64_t)a.B * a.T * a.Hq * (D / 4) * GS + 255) / 256;
+  if (grid > INT_MAX || join > INT_MAX) return hipErrorInvalidValue;
+  const dim3 g((unsigned)grid);
+  switch (p.W) {
+    case 0: hipLaunchKernelGGL((attn_kv_keys<KT, D, 8>), g, dim3(512), 0, s, a, p.NS, p.least); break;
+    case 2: hipLaunchKernelGGL((attn_kv_rows<KT, D, 2>), g, dim3(128), 0, s, a, p.NS, p.least, p.RB); break;
+    case 4: hipLaunchKernelGGL((attn_kv_rows<KT, D, 4>), g, dim3(256), 0, s, a, p.NS, p.least, p.RB); break;
+    default: hipLaunchKernelGGL((attn_kv_rows<KT, D, 8>), g, dim3(512), 0, s, a, p.NS, p.least, p.RB);
   }
+  if (p.least && GS == 8)
+    hipLaunchKernelGGL((attn_kv_join<D, 8>), dim3((unsigned)join), dim3(256), 0, s, a, p.RB, 32 * std::max(1, p.W));
+  else if (p.least)
+    hipLaunchKernelGGL((attn_kv_join<D, 1>), dim3((unsigned)join), dim3(256), 0, s, a, p.RB, 32 * std::max(1, p.W));
   return hipGetLastError();
 }
 template <int KT>

@@ -13,7 +13,8 @@ bool view_of(const mtts_kv_cache* c, KvView* v, const char** why) {
   if (!c || !c->k || !c->v) *why = "cache required";
   else if (c->type != KV_BF16 && c->type != KV_E4M3 && c->type != KV_INT8) *why = "cache type is bf16, e4m3 or int8";
   else if (c->type != KV_BF16 && (!c->k_scale || !c->v_scale)) *why = "an 8-bit cache needs its scales";
-  else if (c->rows < 1 || c->n_kv < 1 || c->slots < 32 || c->slots % 32) *why = "cache rows, heads and slots (a multiple of 32)";
+  else if (c->rows < 1 || c->n_kv < 1 || c->slots < 32 || c->slots % 32 || c->slots >= 1 << 25)
+    *why = "cache rows, heads and slots (a multiple of 32, below 2^25)";
   else if (((uintptr_t)c->k | (uintptr_t)c->v | (uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & 15)
     *why = "cache pointers are 16-byte aligned";
   if (*why) return false;

@@ -55,20 +55,16 @@ def _need(cond, what):
         raise ValueError(what)
 
 
-class _On:
-    """the launches of a call go to the device that its tensors are on"""
-    __slots__ = ("dev",)
-
-    def __init__(self, index):
-        self.dev = None if torch.cuda.current_device() == index else torch.cuda.device(index)
-
-    def __enter__(self):
-        if self.dev is not None:
-            self.dev.__enter__()
-
-    def __exit__(self, *e):
-        if self.dev is not None:
-            self.dev.__exit__(*e)
+def _call(name, fn, index, *args):
+    """a launch on torch's current stream of the device that the call's tensors are on"""
+    # (the raw handle: building a Stream object for each call costs as much as the launch)
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        N.check(rc, name)
 
 
 def _device(device):
@@ -101,6 +97,7 @@ class Rope:
         self.turns = turns.to(self.device).contiguous()
         self._c = N.MttsRope(self.turns.data_ptr(), self.rotary_dim, int(self.interleaved), self.factor)
         self._ref = ctypes.addressof(self._c)
+        self._fn = N.load().mtts_k_rope
 
     def apply(self, x: torch.Tensor, positions: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """x bf16 [M, H, head_dim] (any strides between tokens and heads) at int32 positions [M];
@@ -108,20 +105,16 @@ class Rope:
         _need(x.dim() == 3 and x.dtype == torch.bfloat16 and x.shape[2] == self.head_dim and x.device == self.device,
               "x is bf16 [tokens, heads, head_dim] on the frequencies' device")
         M, H, D = x.shape
-        _i32(positions, (M,), self.device, "positions")
+        xs = x.stride()
         if out is None:
-            out = torch.empty((M, H, D), dtype=x.dtype, device=x.device)
+            out, ys = torch.empty((M, H, D), dtype=torch.bfloat16, device=self.device), (H * D, D, 1)
         else:
             _need(out.shape == x.shape and out.dtype == x.dtype and out.device == x.device, "out is like x")
-        _need(x.stride(2) == 1 and out.stride(2) == 1, "a head's dims lie side by side")
-        with _On(self.device.index):
-            N.call("mtts_k_rope", x.data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
-                   positions.data_ptr(), M, H, D, self._ref, _stream(self.device))
+            ys = out.stride()
+        _need(xs[2] == 1 and ys[2] == 1, "a head's dims lie side by side")
+        _call("rope", self._fn, self.device.index, x.data_ptr(), xs[0], xs[1], out.data_ptr(), ys[0], ys[1],
+              _i32(positions, (M,), self.device, "positions"), M, H, D, self._ref)
         return out
-
-
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
 
 
 def _i32(t, shape, device, what):
@@ -175,6 +168,9 @@ class KVCache:
                                 None if self.v_scale is None else self.v_scale.data_ptr(), DTYPES[dtype], rows, n_kv,
                                 head_dim, self.slots)
         self._ref = ctypes.addressof(self._c)
+        L = N.load()
+        self._f_append, self._f_read, self._f_compact = L.mtts_k_kv_append, L.mtts_k_kv_read, L.mtts_k_kv_compact
+        self._f_attn, self._f_ws = L.mtts_k_attn_kv, L.mtts_k_attn_kv_ws_bytes
 
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale) if t is not None)
@@ -196,12 +192,11 @@ class KVCache:
     def _append(self, q, k, v, out, n_heads, ld, B, S, start, rope, positions, counts, q_norm, k_norm, eps):
         if rope is not None:
             _need(rope.head_dim == self.head_dim and rope.device == self.device, "rope is of another head or device")
-        with _On(self.device.index):
-            N.call("mtts_k_kv_append", self._ref, q, ld[0], k, ld[1], v, ld[2],
-                   None if out is None else out.data_ptr(), n_heads * self.head_dim, n_heads,
-                   self._norm(q_norm, "q_norm"), self._norm(k_norm, "k_norm"), eps, None if rope is None else rope._ref,
-                   None if positions is None else _i32(positions, (B, S), self.device, "positions"),
-                   self._start(start, B), self._counts(counts, B), B, S, _stream(self.device))
+        _call("append", self._f_append, self.device.index, self._ref, q, ld[0], k, ld[1], v, ld[2],
+              None if out is None else out.data_ptr(), n_heads * self.head_dim, n_heads, self._norm(q_norm, "q_norm"),
+              self._norm(k_norm, "k_norm"), eps, None if rope is None else rope._ref,
+              None if positions is None else _i32(positions, (B, S), self.device, "positions"), self._start(start, B),
+              self._counts(counts, B), B, S)
 
     def append(self, qkv: torch.Tensor, start: torch.Tensor, n_heads: int, rope: Optional[Rope] = None,
                positions: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None,
@@ -252,9 +247,8 @@ class KVCache:
         _need(B <= self.rows, f"{B} rows for a cache of {self.rows}")
         k = torch.empty((B, self.n_kv, n, self.head_dim), dtype=torch.bfloat16, device=self.device)
         v = torch.empty_like(k)
-        with _On(self.device.index):
-            N.call("mtts_k_kv_read", self._ref, k.data_ptr(), v.data_ptr(), None if start is None else self._start(start, B),
-                   self._counts(counts, B), B, n, _stream(self.device))
+        _call("read", self._f_read, self.device.index, self._ref, k.data_ptr(), v.data_ptr(),
+              None if start is None else self._start(start, B), self._counts(counts, B), B, n)
         return k, v
 
     def compact(self, start: torch.Tensor, path: torch.Tensor, accepted: torch.Tensor) -> None:
@@ -262,9 +256,8 @@ class KVCache:
         path[b, i] holds, for i < accepted[b] (path int32 [B, P], P <= 64; accepted int32 [B])."""
         _need(path.dim() == 2, "path: int32 [B, P]")
         B, P = path.shape
-        with _On(self.device.index):
-            N.call("mtts_k_kv_compact", self._ref, self._start(start, B), _i32(path, (B, P), self.device, "path"),
-                   _i32(accepted, (B,), self.device, "accepted"), B, P, _stream(self.device))
+        _call("compact", self._f_compact, self.device.index, self._ref, self._start(start, B),
+              _i32(path, (B, P), self.device, "path"), _i32(accepted, (B,), self.device, "accepted"), B, P)
 
     def attend(self, q: torch.Tensor, start: torch.Tensor, tree: Optional[torch.Tensor] = None,
                counts: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None, scale: Optional[float] = None,
@@ -293,12 +286,11 @@ class KVCache:
                   "out: contiguous, like q")
         _need(scale is None or scale > 0, "scale > 0")
         n = 0 if max_len is None else max(1, int(max_len))
-        L = N.load()
-        with _On(self.device.index):
-            need = L.mtts_k_attn_kv_ws_bytes(B, T, H, self.n_kv, D, self.slots, n)
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-            N.check(L.mtts_k_attn_kv(self._ref, q.data_ptr(), ldq, out.data_ptr(), H * D, H, self._start(start, B),
-                                     self._counts(counts, B), None if tree is None else tree.data_ptr(),
-                                     None if mask is None else mask.data_ptr(), B, T, 0.0 if scale is None else scale, n,
-                                     None if ws is None else ws.data_ptr(), _stream(self.device)), "attend")
+        need = self._f_ws(B, T, H, self.n_kv, D, self.slots, n)
+        # (scratch of this call alone, from torch's allocator: in order on this stream, a graph's own in a capture)
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        _call("attend", self._f_attn, self.device.index, self._ref, q.data_ptr(), ldq, out.data_ptr(), H * D, H,
+              self._start(start, B), self._counts(counts, B), None if tree is None else tree.data_ptr(),
+              None if mask is None else mask.data_ptr(), B, T, 0.0 if scale is None else scale, n,
+              None if ws is None else ws.data_ptr())
         return out
