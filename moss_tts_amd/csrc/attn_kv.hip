@@ -43,25 +43,23 @@ __device__ __forceinline__ RowLen row_len(const AttnKvArgs& a, int b) {
 // of a longer one every block leaves a partial (m, l, o), in slot 2 x + 1 if the row begins in it and
 // 2 x if it began before, and the join adds them up in order: the first block and the number of blocks of
 // each row stand at the head of the workspace.  share 0: a block a row, nothing to join.
+// A segment more costs a block about SEG tiles (its loads start anew), so a row counts for SEG more.
 __device__ __forceinline__ int tiles_of(const RowLen& r) { return r.n ? (r.nk + 31) >> 5 : 0; }
-__device__ __forceinline__ int wave_isum(int v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return __builtin_amdgcn_readfirstlane(v);
-}
-__device__ __forceinline__ int wave_iscan(int v, int lane) {  // sum up to and with this lane
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(v, o, 64);
-    if (lane >= o) v += u;
-  }
+// sum up to and with this lane: rows of 16 lanes by shifts, then the rows' sums by broadcasts
+__device__ __forceinline__ int wave_iscan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // lane 15 of rows 0 and 2 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // lane 31 into rows 2 and 3
   return v;
 }
 struct Seg {
   int b, t0, t1, slot;  // tiles [t0, t1) of row b; slot -1: the whole row
   RowLen len;
 };
-template <class F>
+template <int SEG, class F>
 __device__ __forceinline__ void for_segments(const AttnKvArgs& a, int NS, int least, int x, bool head, F&& body) {
   if (least == 0) {
     const RowLen r = row_len(a, x);
@@ -69,23 +67,29 @@ __device__ __forceinline__ void for_segments(const AttnKvArgs& a, int NS, int le
     return;
   }
   const int lane = threadIdx.x & 63;
-  int total = 0;
+  int total = 0, run = 0, upto = 0;
   RowLen r{0, 0, 0};
   for (int b0 = (a.B - 1) & ~63; b0 >= 0; b0 -= 64) {
     r = b0 + lane < a.B ? row_len(a, b0 + lane) : RowLen{0, 0, 0};
-    total += wave_isum(tiles_of(r));
+    run = tiles_of(r) ? tiles_of(r) + SEG : 0;
+    upto = wave_iscan(run);
+    total += __builtin_amdgcn_readlane(upto, 63);
   }
   const int share = max(least, (total + NS - 1) / NS);
   const int64_t lo = (int64_t)x * share, hi = lo + share;
   int off = 0;
   for (int b0 = 0; b0 < a.B && (off < hi || head); b0 += 64) {
-    if (b0) r = b0 + lane < a.B ? row_len(a, b0 + lane) : RowLen{0, 0, 0};
-    const int nt = tiles_of(r), end = off + wave_iscan(nt, lane), beg = end - nt;
+    if (b0) {
+      r = b0 + lane < a.B ? row_len(a, b0 + lane) : RowLen{0, 0, 0};
+      run = tiles_of(r) ? tiles_of(r) + SEG : 0;
+      upto = wave_iscan(run);
+    }
+    const int end = off + upto, beg = run ? end - run + SEG : end;  // the row's tiles are [beg, end) of the run
     if (head && threadIdx.x < 64 && b0 + lane < a.B) {
-      const int x0 = nt ? beg / share : 0, ns = nt ? (end - 1) / share - x0 + 1 : 0;
+      const int x0 = beg / share, ns = run ? (end - 1) / share - x0 + 1 : 0;
       *reinterpret_cast<int2*>(a.part + 2 * (b0 + lane)) = make_int2(x0, ns);
     }
-    uint64_t hit = __ballot(nt > 0 && beg < hi && end > lo);
+    uint64_t hit = __ballot(beg < end && beg < hi && end > lo);
     while (hit) {
       const int f = __ffsll((unsigned long long)hit) - 1;
       hit &= hit - 1;
@@ -253,8 +257,9 @@ struct RowState {
     // m follows the maximum only once that has outgrown it by 2^8: p stays below 256, which costs no bit of
     // it, and the 16 D / 32 products of the output's rescaling are rare (at each new maximum of any of 32
     // rows they were two fifths of the loop)
-    if (__any(mx > m + 8.f)) {
-      const float mn = fmaxf(m, mx);
+    const bool up = mx > m + 8.f;  // (each row for itself: its result is the same whatever rows it shares a wave with)
+    if (__any(up)) {
+      const float mn = up ? mx : m;
       const float al = m == -INFINITY ? (mn == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
       l *= al;
@@ -504,7 +509,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_kv_keys(AttnKvArgs a, int NS,
   const uint32_t sl = 16 * ((lane & 15) >> 3) + 8 * h + (lane & 7);  // the slot whose scales this lane holds
   char* mylds = lds + wave * WL;
 
-  for_segments(a, NS, least, pl.x, blockIdx.x == 0, [&](const Seg& sg) {
+  for_segments<16>(a, NS, least, pl.x, blockIdx.x == 0, [&](const Seg& sg) {
     const int b = sg.b;
     const RowLen len = sg.len;
     const int R = len.n * G;
@@ -678,7 +683,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv_rows(AttnKvArgs a, int NS,
   if (pl.unit >= NS * Hkv) return;
   const float c = a.scale * 1.44269504088896340736f;
 
-  for_segments(a, NS, least, pl.x, blockIdx.x == 0, [&](const Seg& sg) {
+  for_segments<6>(a, NS, least, pl.x, blockIdx.x == 0, [&](const Seg& sg) {
     const int b = sg.b;
     const RowLen len = sg.len;
     const int r0 = pl.rb * rows, Rend = min(len.n * G, r0 + rows);  // this block's rows of (row, KV head)
@@ -698,6 +703,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv_rows(AttnKvArgs a, int NS,
     // A turn works on TT tiles out of one half of LDS, while the next TT go from registers into the other
     // half and the TT behind them are loaded: what a turn waits for was asked for a whole turn ago.
     St gk[TT], gv[TT];
+    const int wv = W - 1 - wave;  // (a tile of fewer loads than waves: K by the first waves, V by the last)
     float ks[TT], vs[TT], kn[TT], vn[TT];  // scales of this turn's tiles and of the next one's
     const uint32_t at = h * FB + n * 16;
     auto fetch = [&](int tile) {
@@ -706,14 +712,14 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv_rows(AttnKvArgs a, int NS,
         const int t = min(tile + i, t1 - 1);  // (past the end the last tile again: in bounds, not used)
         gk[i].load_scales(a, head, t, lane);
         gk[i].load_k(kb, t, wave, lane);
-        gv[i].load_v(vb, slots, t, wave, lane);
+        gv[i].load_v(vb, slots, t, wv, lane);
       }
     };
     auto put = [&](int tile, int half) {
 #pragma unroll
       for (int i = 0; i < TT; ++i) {
         gk[i].store_k(wave, lane, lk[half][i]);
-        if (gv[i].store_v(a, b, len, min(tile + i, t1 - 1), wave, lane, lv[half][i])) spared = 1;
+        if (gv[i].store_v(a, b, len, min(tile + i, t1 - 1), wv, lane, lv[half][i])) spared = 1;
         if constexpr (Q8) {
           kn[i] = gk[i].ks * c;
           vn[i] = gk[i].vs;
@@ -905,7 +911,7 @@ static AkvPlan plan(int B, int T, int Hq, int n_kv, int slots, int max_len) {
   const int64_t tiles = (len + 31) / 32;                              // of the longest row
   const int64_t units = std::max<int64_t>(1, (int64_t)n_kv * p.RB);   // blocks a row, unsplit
   const int64_t room = 256 * (p.W == 0 ? 1 : 8 / p.W);                // blocks that the card holds at once
-  const int64_t most = p.W == 0 ? 32 : 8, least = p.W == 0 ? 8 : 4;
+  const int64_t most = p.W == 0 ? 64 : p.W == 8 ? 20 : p.W == 4 ? 12 : 8, least = p.W == 0 || p.W == 2 ? 8 : 4;
   p.least = (int)least;
   p.NS = (int)std::max<int64_t>(1, std::min(room / units, (int64_t)B * ((tiles + least - 1) / least)));
   // short rows, or enough of them: nothing to join
