@@ -59,52 +59,70 @@ struct Seg {
   int b, t0, t1, slot;  // tiles [t0, t1) of row b; slot -1: the whole row
   RowLen len;
 };
-template <int SEG, class F>
-__device__ __forceinline__ void for_segments(const AttnKvArgs& a, int NS, int least, int x, bool head, F&& body) {
-  if (least == 0) {
-    const RowLen r = row_len(a, x);
-    body(Seg{x, 0, INT_MAX, -1, r});
-    return;
-  }
-  const int lane = threadIdx.x & 63;
-  int total = 0, run = 0, upto = 0;
-  RowLen r{0, 0, 0};
-  for (int b0 = (a.B - 1) & ~63; b0 >= 0; b0 -= 64) {
+template <int SEG>
+struct Segments {
+  const AttnKvArgs& a;
+  RowLen r;
+  int64_t lo, hi;
+  uint64_t hit;
+  int x, b0, beg, end, off, lane;
+  bool direct;
+
+  __device__ __forceinline__ void rows_at(int from) {  // 64 rows: their lengths, their places in the run
+    b0 = from;
     r = b0 + lane < a.B ? row_len(a, b0 + lane) : RowLen{0, 0, 0};
-    run = tiles_of(r) ? tiles_of(r) + SEG : 0;
-    upto = wave_iscan(run);
-    total += __builtin_amdgcn_readlane(upto, 63);
+    const int t = tiles_of(r), run = t ? t + SEG : 0;
+    end = off + wave_iscan(run);
+    beg = end - t;
   }
-  const int share = max(least, (total + NS - 1) / NS);
-  const int64_t lo = (int64_t)x * share, hi = lo + share;
-  int off = 0;
-  for (int b0 = 0; b0 < a.B && (off < hi || head); b0 += 64) {
-    if (b0) {
-      r = b0 + lane < a.B ? row_len(a, b0 + lane) : RowLen{0, 0, 0};
-      run = tiles_of(r) ? tiles_of(r) + SEG : 0;
-      upto = wave_iscan(run);
+  __device__ __forceinline__ Segments(const AttnKvArgs& a, int NS, int least, int x, bool head)
+      : a(a), r{0, 0, 0}, hit(1), x(x), b0(0), beg(0), end(0), off(0), lane(threadIdx.x & 63), direct(least == 0) {
+    if (direct) return;
+    int total = 0;
+    for (int from = (a.B - 1) & ~63; from >= 0; from -= 64) {
+      rows_at(from);
+      total += __builtin_amdgcn_readlane(end, 63);
     }
-    const int end = off + upto, beg = run ? end - run + SEG : end;  // the row's tiles are [beg, end) of the run
-    if (head && threadIdx.x < 64 && b0 + lane < a.B) {
-      const int x0 = beg / share, ns = run ? (end - 1) / share - x0 + 1 : 0;
-      *reinterpret_cast<int2*>(a.part + 2 * (b0 + lane)) = make_int2(x0, ns);
-    }
-    uint64_t hit = __ballot(beg < end && beg < hi && end > lo);
-    while (hit) {
-      const int f = __ffsll((unsigned long long)hit) - 1;
-      hit &= hit - 1;
-      const int sb = __builtin_amdgcn_readlane(beg, f), se = __builtin_amdgcn_readlane(end, f);
-      Seg g;
-      g.b = b0 + f;
-      g.t0 = (int)max(lo, (int64_t)sb) - sb;
-      g.t1 = (int)min(hi, (int64_t)se) - sb;
-      g.slot = sb >= lo && se <= hi ? -1 : 2 * x + (sb >= lo ? 1 : 0);
-      g.len = RowLen{__builtin_amdgcn_readlane(r.start, f), __builtin_amdgcn_readlane(r.n, f), __builtin_amdgcn_readlane(r.nk, f)};
-      body(g);
-    }
-    off = __builtin_amdgcn_readlane(end, 63);
+    const int share = max(least, (total + NS - 1) / NS);
+    lo = (int64_t)x * share;
+    hi = lo + share;
+    if (head)
+      for (int from = 0; from < a.B; from += 64) {
+        if (from) rows_at(from);
+        if (threadIdx.x < 64 && b0 + lane < a.B) {
+          const int x0 = beg / share, ns = beg < end ? (end - 1) / share - x0 + 1 : 0;
+          *reinterpret_cast<int2*>(a.part + 2 * (b0 + lane)) = make_int2(x0, ns);
+        }
+        off = __builtin_amdgcn_readlane(end, 63);
+      }
+    off = 0;
+    if (head && a.B > 64) rows_at(0);
+    hit = __ballot(beg < end && beg < hi && end > lo);
   }
-}
+  __device__ __forceinline__ bool next(Seg& g) {
+    if (direct) {
+      if (!hit) return false;
+      hit = 0;
+      g = Seg{x, 0, INT_MAX, -1, row_len(a, x)};
+      return true;
+    }
+    while (!hit) {
+      off = __builtin_amdgcn_readlane(end, 63);
+      if (b0 + 64 >= a.B || off >= hi) return false;
+      rows_at(b0 + 64);
+      hit = __ballot(beg < end && beg < hi && end > lo);
+    }
+    const int f = __ffsll((unsigned long long)hit) - 1;
+    hit &= hit - 1;
+    const int sb = __builtin_amdgcn_readlane(beg, f), se = __builtin_amdgcn_readlane(end, f);
+    g.b = b0 + f;
+    g.t0 = (int)max(lo, (int64_t)sb) - sb;
+    g.t1 = (int)min(hi, (int64_t)se) - sb;
+    g.slot = sb >= lo && se <= hi ? -1 : 2 * x + (sb >= lo ? 1 : 0);
+    g.len = RowLen{__builtin_amdgcn_readlane(r.start, f), __builtin_amdgcn_readlane(r.n, f), __builtin_amdgcn_readlane(r.nk, f)};
+    return true;
+  }
+};
 // floats at the head of the workspace
 __host__ __device__ __forceinline__ size_t head_floats(int B) { return ((size_t)2 * B + 63) / 64 * 64; }
 
@@ -383,11 +401,8 @@ __device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70
 
 // this lane's row r: token, tree word, and the q fragments (16-byte pieces of dims 32 j + 16 h + 8 e)
 template <int D>
-__device__ __forceinline__ Row load_row(const AttnKvArgs& a, int b, int hkv, const RowLen& len, int r, int R, int h,
+__device__ __forceinline__ Row load_row(const AttnKvArgs& a, int b, int hkv, const RowLen& len, int G, int t, int g, int h,
                                         bf16x8* qf) {
-  const int G = a.Hq / a.c.n_kv;
-  const bool on = r < R;
-  const int t = on ? r / G : 0, g = on ? r - t * G : 0;
   const bf16_t* q = a.q + ((size_t)b * a.T + t) * a.ldq + (size_t)(hkv * G + g) * D + h * 16;
 #pragma unroll
   for (int j = 0; j < D / 32; ++j)
@@ -492,7 +507,7 @@ struct Stage {
 // block take tiles in turn, loaded one tile ahead, with no barrier in the loop, and merge once at the
 // end.  8-bit fragments go from memory straight into registers, bf16 ones through LDS of the wave's own.
 template <int KT, int D, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void attn_kv_keys(AttnKvArgs a, int NS, int least) {
+__global__ __launch_bounds__(64 * NW, 2) void attn_kv_keys(AttnKvArgs a, int NS, int least, uint32_t rG) {
   constexpr bool Q8 = KT != KV_BF16;
   constexpr int NF = D / 32;
   constexpr int DT = D / 32;
@@ -503,48 +518,63 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_kv_keys(AttnKvArgs a, int NS,
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, h = lane >> 5;
   const int Hkv = a.c.n_kv, G = a.Hq / Hkv, slots = a.c.slots;
-  const Place pl = place_of(NS, least, 1, Hkv);
-  if (pl.unit >= NS * Hkv) return;
+  const int hkv = blockIdx.x, x = blockIdx.y;
   const float c = a.scale * 1.44269504088896340736f;  // softmax in powers of two
   const uint32_t sl = 16 * ((lane & 15) >> 3) + 8 * h + (lane & 7);  // the slot whose scales this lane holds
   char* mylds = lds + wave * WL;
 
-  for_segments<16>(a, NS, least, pl.x, blockIdx.x == 0, [&](const Seg& sg) {
-    const int b = sg.b;
-    const RowLen len = sg.len;
-    const int R = len.n * G;
-    if (R == 0) return;
-    const int t1 = min(sg.t1, (len.nk + 31) >> 5);
-    int tile = sg.t0 + wave;
-    const size_t head = ((size_t)b * Hkv + pl.hkv) * slots;
-    const char* kb = (const char*)a.c.k + head * D * (Q8 ? 1 : 2);
-    const char* vb = (const char*)a.c.v + head * D * (Q8 ? 1 : 2);
-    u32x4 kf[NF], vf[NF];  // 8-bit
-    St sk, sv;             // bf16
-    float ksn = 0.f, vsn = 0.f;
-    auto load_k = [&](int t) {
-      const char* p = kb + (size_t)t * (32 * D);
+  const char *kb, *vb;
+  size_t head;
+  u32x4 kf[NF], vf[NF];  // 8-bit
+  St sk, sv;             // bf16
+  float ksn = 0.f, vsn = 0.f;
+  auto row_at = [&](int b) {
+    head = ((size_t)b * Hkv + hkv) * slots;
+    kb = (const char*)a.c.k + head * D * (Q8 ? 1 : 2);
+    vb = (const char*)a.c.v + head * D * (Q8 ? 1 : 2);
+  };
+  auto load_k = [&](int t) {
+    const char* p = kb + (size_t)t * (32 * D);
 #pragma unroll
       for (int j = 0; j < NF; ++j) kf[j] = *reinterpret_cast<const u32x4*>(p + (uint32_t)(j * 1024 + lane * 16));
       ksn = (a.c.ks + head + t * 32)[sl];
       vsn = (a.c.vs + head + t * 32)[sl];
     };
-    auto load_v = [&](int t) {
-      const char* p = vb + (size_t)t * (32 * D);
+  auto load_v = [&](int t) {
+    const char* p = vb + (size_t)t * (32 * D);
 #pragma unroll
-      for (int j = 0; j < NF; ++j) vf[j] = *reinterpret_cast<const u32x4*>(p + (uint32_t)(j * 1024 + lane * 16));
-    };
-    if (tile < t1) {
-      if constexpr (Q8) {
-        load_k(tile);
-        load_v(tile);
-      } else {
-        sk.load_k(kb, tile, 0, lane);
-        sv.load_v(vb, slots, tile, 0, lane);
-      }
+    for (int j = 0; j < NF; ++j) vf[j] = *reinterpret_cast<const u32x4*>(p + (uint32_t)(j * 1024 + lane * 16));
+  };
+  auto load_tile = [&](int t) {
+    if constexpr (Q8) {
+      load_k(t);
+      load_v(t);
+    } else {
+      sk.load_k(kb, t, 0, lane);
+      sv.load_v(vb, slots, t, 0, lane);
+    }
+  };
+  // an unsplit row's first tiles are known before its length is (and there, whatever that turns out to be;
+  // 8-bit: bf16 has no registers left for it)
+  if (Q8 && least == 0) {
+    row_at(x);
+    load_tile(min(wave, (slots >> 5) - 1));
+  }
+  Segments<16> it(a, NS, least, x, hkv == 0 && x == 0);
+  for (Seg sg; it.next(sg);) {
+    const int b = sg.b;
+    const RowLen len = sg.len;
+    const int R = len.n * G;
+    if (R == 0) continue;
+    const int t1 = min(sg.t1, (len.nk + 31) >> 5);
+    int tile = sg.t0 + wave;
+    if (!Q8 || least) {
+      row_at(b);
+      if (tile < t1) load_tile(tile);
     }
     bf16x8 qf[D / 16];
-    const Row row = load_row<D>(a, b, pl.hkv, len, n, R, h, qf);
+    const int tk = n < R ? n * rG >> 16 : 0;  // n / G, exact for n and G of at most 32
+    const Row row = load_row<D>(a, b, hkv, len, G, tk, n < R ? n - tk * G : 0, h, qf);
     RowState<KT, D> st;
     st.clear();
     bool spared = false;
@@ -617,22 +647,6 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_kv_keys(AttnKvArgs a, int NS,
       mls[wave][n][0] = st.m;
       mls[wave][n][1] = st.l;
     }
-    __syncthreads();
-    float M = -INFINITY, L = 0.f, mine = 0.f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) M = fmaxf(M, mls[w][n][0]);
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float mw = mls[w][n][0];
-      const float f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - M);
-      L += mls[w][n][1] * f;
-      if (w == wave) mine = f;
-    }
-    // (a row that saw nothing is 0; a whole row is divided here, a split one by the join)
-    const bool whole = sg.slot < 0;
-    const float sc = !whole ? mine : L == 0.f ? 0.f : mine / L;
-    float* po = a.part + head_floats(a.B) + (size_t)(sg.slot * Hkv + pl.hkv) * 32 * (D + 2);
-    if (!whole && wave == 0 && h == 0) *reinterpret_cast<float2*>(po + 32 * D + n * 2) = make_float2(M, L);
     float* os = reinterpret_cast<float*>(mylds) + n * (D + 4) + 4 * h;
     if (n < R) {
 #pragma unroll
@@ -640,28 +654,37 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_kv_keys(AttnKvArgs a, int NS,
 #pragma unroll
         for (int i = 0; i < 16; i += 4)
           *reinterpret_cast<float4*>(os + 32 * t + 2 * i) =
-              make_float4(st.o[t][i] * sc, st.o[t][i + 1] * sc, st.o[t][i + 2] * sc, st.o[t][i + 3] * sc);
+              make_float4(st.o[t][i], st.o[t][i + 1], st.o[t][i + 2], st.o[t][i + 3]);
     }
     __syncthreads();
+    const bool whole = sg.slot < 0;
+    float* po = a.part + head_floats(a.B) + (size_t)(sg.slot * Hkv + hkv) * 32 * (D + 2);
     for (int q = threadIdx.x; q < R * (D / 4); q += 64 * NW) {
       const int r = q / (D / 4), d = q % (D / 4) * 4;
       const char* src = lds + (r * (D + 4) + d) * 4;
-      float4 y = *reinterpret_cast<const float4*>(src);
+      float M = -INFINITY, L = 0.f;
 #pragma unroll
-      for (int w = 1; w < NW; ++w) {
+      for (int w = 0; w < NW; ++w) M = fmaxf(M, mls[w][r][0]);
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float mw = mls[w][r][0], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - M);
         const float4 z = *reinterpret_cast<const float4*>(src + w * WL);
-        y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
+        L += f * mls[w][r][1];
+        y.x += f * z.x; y.y += f * z.y; y.z += f * z.z; y.w += f * z.w;
       }
-      if (!whole) {
+      if (!whole) {  // a split row is divided by the join
         *reinterpret_cast<float4*>(po + r * D + d) = y;
+        if (d == 0) *reinterpret_cast<float2*>(po + 32 * D + r * 2) = make_float2(M, L);
       } else {
-        const int tk = r / G;
-        bf16_t* dst = a.out + ((size_t)b * a.T + tk) * a.ldo + (size_t)(pl.hkv * G + r - tk * G) * D + d;
-        *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(y.x, y.y), pack2(y.z, y.w));
+        const float sc = L == 0.f ? 0.f : 1.f / L;  // (a row that saw nothing is 0)
+        const int t = r * rG >> 16;
+        bf16_t* dst = a.out + ((size_t)b * a.T + t) * a.ldo + (size_t)(hkv * G + r - t * G) * D + d;
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(y.x * sc, y.y * sc), pack2(y.z * sc, y.w * sc));
       }
     }
     if (least) __syncthreads();  // (the next segment writes LDS)
-  });
+  }
 }
 
 // More rows: bound by the arithmetic on the scores.  The W waves of a block, 32 rows each, go through the
@@ -683,11 +706,12 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv_rows(AttnKvArgs a, int NS,
   if (pl.unit >= NS * Hkv) return;
   const float c = a.scale * 1.44269504088896340736f;
 
-  for_segments<6>(a, NS, least, pl.x, blockIdx.x == 0, [&](const Seg& sg) {
+  Segments<6> it(a, NS, least, pl.x, blockIdx.x == 0);
+  for (Seg sg; it.next(sg);) {
     const int b = sg.b;
     const RowLen len = sg.len;
     const int r0 = pl.rb * rows, Rend = min(len.n * G, r0 + rows);  // this block's rows of (row, KV head)
-    if (r0 >= Rend) return;
+    if (r0 >= Rend) continue;
     // a chain's row block sees no slot behind its last token's
     const int nk = a.tree ? len.nk : min(len.nk, len.start + (Rend - 1) / G + 1);
     const int t0 = sg.t0, t1 = min(sg.t1, (nk + 31) >> 5);
@@ -728,7 +752,8 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv_rows(AttnKvArgs a, int NS,
     };
     if (t0 < t1) fetch(t0);
     bf16x8 qf[D / 16];
-    const Row row = load_row<D>(a, b, pl.hkv, len, myr, Rend, h, qf);
+    const int tk = myr < Rend ? myr / G : 0;
+    const Row row = load_row<D>(a, b, pl.hkv, len, G, tk, myr < Rend ? myr - tk * G : 0, h, qf);
     __syncthreads();  // (spared is 0, and the last segment's tiles have been read)
     loads_done();
     if (t0 < t1) {
@@ -798,7 +823,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv_rows(AttnKvArgs a, int NS,
       if (least) __syncthreads();  // (the next segment clears it)
     }
     st.l = half_sum(st.l);
-    if (myr >= Rend) return;
+    if (myr >= Rend) continue;
     if (sg.slot >= 0) {  // a split row is divided by the join
       float* po = a.part + head_floats(a.B) + ((size_t)(sg.slot * Hkv + pl.hkv) * RB + pl.rb) * rows * (D + 2);
       const int rr = wave * 32 + n;
@@ -819,7 +844,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv_rows(AttnKvArgs a, int NS,
           *reinterpret_cast<uint2*>(dst + 32 * t + 2 * i + 4 * h) =
               make_uint2(pack2(st.o[t][i] * sc, st.o[t][i + 1] * sc), pack2(st.o[t][i + 2] * sc, st.o[t][i + 3] * sc));
     }
-  });
+  }
 }
 
 // Joins the partials of a row: GS groups of D / 4 threads (4 dims each) take every GS-th block's partial,
@@ -933,10 +958,14 @@ static hipError_t launch(const AttnKvArgs& a, const AkvPlan& p, hipStream_t s) {
   const int64_t grid = ((int64_t)p.NS * a.c.n_kv + 7) / 8 * 8 * p.RB;
   const int GS = p.NS > 4 * a.B ? 8 : 1;  // (rows of many partials: they are read at once, not one after the other)
   const int64_t join = ((int64_t)a.B * a.T * a.Hq * (D / 4) * GS + 255) / 256;
-  if (grid > INT_MAX || join > INT_MAX) return hipErrorInvalidValue;
+  if (grid > INT_MAX || join > INT_MAX || (p.W == 0 && p.NS > 65535)) return hipErrorInvalidValue;
   const dim3 g((unsigned)grid);
   switch (p.W) {
-    case 0: hipLaunchKernelGGL((attn_kv_keys<KT, D, 8>), g, dim3(512), 0, s, a, p.NS, p.least); break;
+    case 0: {
+      const uint32_t G = a.Hq / a.c.n_kv, rG = (65536 + G - 1) / G;
+      hipLaunchKernelGGL((attn_kv_keys<KT, D, 8>), dim3(a.c.n_kv, p.NS), dim3(512), 0, s, a, p.NS, p.least, rG);
+      break;
+    }
     case 2: hipLaunchKernelGGL((attn_kv_rows<KT, D, 2>), g, dim3(128), 0, s, a, p.NS, p.least, p.RB); break;
     case 4: hipLaunchKernelGGL((attn_kv_rows<KT, D, 4>), g, dim3(256), 0, s, a, p.NS, p.least, p.RB); break;
     default: hipLaunchKernelGGL((attn_kv_rows<KT, D, 8>), g, dim3(512), 0, s, a, p.NS, p.least, p.RB);

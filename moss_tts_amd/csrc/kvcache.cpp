@@ -148,6 +148,7 @@ extern "C" int mtts_k_attn_kv(const mtts_kv_cache* cache, const uint16_t* q, siz
   if (!q || !out || !start) return fail(MTTS_E_INVALID, "attention: missing arguments");
   if (((uintptr_t)q & 15) || ldq % 8 || ((uintptr_t)out & 7) || ldo % 4 || ((uintptr_t)mask & 7) || ((uintptr_t)tree & 7))
     return fail(MTTS_E_INVALID, "attention: q 16-byte and out 8-byte aligned, in every row; mask and tree 8-byte");
+  if (B > 65535) return fail(MTTS_E_UNSUPPORTED, "attention: at most 65,535 rows");
   if ((int64_t)T * n_heads > (1 << 30)) return fail(MTTS_E_INVALID, "attention: too many tokens");
   if (!ws && attn_kv_ws_bytes(B, T, n_heads, c.n_kv, c.D, c.slots, max_len))
     return fail(MTTS_E_INVALID, "attention: workspace required");

@@ -188,10 +188,9 @@ __device__ __forceinline__ int row_count(const int* counts, int b, int S) {
 
 // Append.  Three kinds of blocks in one launch:
 //   [0, nq)    q: a wave per (token, run of heads): norm, rotation, q_out
-//   [.., +nk)  k: a wave per (64 / pt tokens of one row, run of heads): norm, rotation, amax over the
-//              head's lanes, codes to the tile
-//   [.., +nv)  v: a block per (row, kv head, tile of 32 slots): codes go through LDS, because a V tile
-//              holds 16 slots of one dim side by side
+//   [.., +nk)  k: a block per (row, kv head, tile of 32 slots): norm, rotation, amax over the head's lanes,
+//              codes through LDS into the tile's order, so that they leave in 16-byte pieces side by side
+//   [.., +nk)  v: the same; a V tile holds 16 slots of one dim side by side
 template <int V>
 __device__ __forceinline__ float head_sum(float s, int pt) {
   for (int o = 1; o < pt; o <<= 1) s += __shfl_xor(s, o, 64);
@@ -234,69 +233,89 @@ __device__ void append_q(const KvAppendArgs& a, int blk, int hpc) {
   }
 }
 
+constexpr int KV_DMAX = 128;
+
+// the tile of 32 slots that K or V block `blk` works on: new tokens at its slots [lo, hi); false: none
+struct KvTile {
+  int b, h, start, lo, hi;
+  int64_t base;  // its first slot
+  size_t head;
+};
+__device__ __forceinline__ bool kv_tile(const KvAppendArgs& a, int blk, KvTile* t) {
+  const int tiles = (a.S + 31) / 32 + 1;  // a row's new slots touch this many tiles at most
+  t->b = blk / (tiles * a.c.n_kv);
+  t->h = blk / tiles % a.c.n_kv;
+  t->start = a.start[t->b];
+  const int64_t end = (int64_t)t->start + row_count(a.counts, t->b, a.S);
+  t->base = ((int64_t)(t->start >> 5) + blk % tiles) * 32;
+  if (t->base < 0 || t->base >= a.c.slots || t->base >= end) return false;
+  t->lo = (int)max((int64_t)0, t->start - t->base);
+  t->hi = (int)min((int64_t)32, end - t->base);
+  t->head = ((size_t)t->b * a.c.n_kv + t->h) * a.c.slots;
+  return true;
+}
+
+// pieces of 2 V dims of one token each
 template <int V>
-__device__ void append_k(const KvAppendArgs& a, int blk, int hpc) {
-  const int D = a.c.D, pt = D / (2 * V), lane = threadIdx.x & 63, c = lane % pt;
-  const int tpw = 64 / pt;  // tokens a wave
-  const int runs = (a.c.n_kv + hpc - 1) / hpc, groups = (a.S + tpw - 1) / tpw;
-  const int64_t w = (int64_t)blk * 4 + (threadIdx.x >> 6);
-  if (w >= (int64_t)a.B * groups * runs) return;
-  const int h0 = (int)(w % runs) * hpc, h1 = min(h0 + hpc, a.c.n_kv);
-  const int b = (int)(w / runs / groups), t = (int)(w / runs % groups) * tpw + lane / pt;
-  const int64_t at = (int64_t)a.start[b] + t;
-  const bool on = t < row_count(a.counts, b, a.S) && at >= 0 && at < a.c.slots;
-  const int slot = on ? (int)at : 0;
-  if (!__any(on)) return;
-  const int m = b * a.S + min(t, a.S - 1);
-  const Chunk<V> ch(a.r, c);
-  float cs[V], sn[V], nw[2 * V];
-  if (ch.rot) rope_angles<V>(a.r, c, a.pos ? a.pos[m] : slot, cs, sn);
-  if (a.kn) load_pieces<V>(a.kn, ch, nw);
-  const bf16_t* src = a.k + (size_t)m * a.ldk;
-  for (int h = h0; h < h1; ++h) {
+__device__ void append_k(const KvAppendArgs& a, int blk, char* lds) {
+  KvTile t;
+  if (!kv_tile(a, blk, &t)) return;
+  const int D = a.c.D, pt = D / (2 * V);
+  for (int i = threadIdx.x; i < 32 * pt; i += 256) {  // (32 pt is a multiple of 64: whole waves)
+    const int j = i / pt, c = i % pt;
+    const bool on = j >= t.lo && j < t.hi;
+    if (!__any(on)) continue;
+    const int64_t slot = t.base + j;
+    const size_t m = (size_t)t.b * a.S + (on ? slot - t.start : 0);
+    const Chunk<V> ch(a.r, c);
     float x[2 * V];
-    load_pieces<V>(src + (size_t)h * D, ch, x);
-    if (a.kn) head_norm<V>(x, nw, pt, D, a.eps);
-    if (ch.rot) rotate<V>(a.r, cs, sn, x);
-    const size_t head = ((size_t)b * a.c.n_kv + h) * a.c.slots;
+    load_pieces<V>(a.k + m * a.ldk + (size_t)t.h * D, ch, x);
+    if (a.kn) {
+      float nw[2 * V];
+      load_pieces<V>(a.kn, ch, nw);
+      head_norm<V>(x, nw, pt, D, a.eps);
+    }
+    if (ch.rot) {
+      float cs[V], sn[V];
+      rope_angles<V>(a.r, c, a.pos ? a.pos[m] : (int)slot, cs, sn);
+      rotate<V>(a.r, cs, sn, x);
+    }
     if (a.c.type == KV_BF16) {
-      if (on) store_pieces<V>((bf16_t*)a.c.k + (head + slot) * D, ch, x);
+      if (on) store_pieces<V>((bf16_t*)a.c.k + (t.head + slot) * D, ch, x);
       continue;
     }
     float am = 0.f;
 #pragma unroll
-    for (int i = 0; i < 2 * V; ++i) am = amax_nan(am, x[i]);
+    for (int k = 0; k < 2 * V; ++k) am = amax_nan(am, x[k]);
     for (int o = 1; o < pt; o <<= 1) am = amax_nan(am, __shfl_xor(am, o, 64));
     const Quant z(am, a.c.type);
-    if (!on) continue;
-    uint8_t* tile = (uint8_t*)a.c.k + (head + (slot & ~31)) * D;
     if constexpr (V == 8) {
-      *reinterpret_cast<uint2*>(tile + kv_k_byte(slot & 31, ch.d0)) =
-          make_uint2(codes4(z, x, a.c.type), codes4(z, x + 4, a.c.type));
-      *reinterpret_cast<uint2*>(tile + kv_k_byte(slot & 31, ch.d1)) =
+      *reinterpret_cast<uint2*>(lds + kv_k_byte(j, ch.d0)) = make_uint2(codes4(z, x, a.c.type), codes4(z, x + 4, a.c.type));
+      *reinterpret_cast<uint2*>(lds + kv_k_byte(j, ch.d1)) =
           make_uint2(codes4(z, x + 8, a.c.type), codes4(z, x + 12, a.c.type));
     } else {
-      tile[kv_k_byte(slot & 31, ch.d0)] = code1(z, x[0], a.c.type);
-      tile[kv_k_byte(slot & 31, ch.d1)] = code1(z, x[1], a.c.type);
+      lds[kv_k_byte(j, ch.d0)] = (char)code1(z, x[0], a.c.type);
+      lds[kv_k_byte(j, ch.d1)] = (char)code1(z, x[1], a.c.type);
     }
-    if (c == 0) a.c.ks[head + slot] = z.scale;
+    if (on && c == 0) a.c.ks[t.head + slot] = z.scale;
+  }
+  if (a.c.type == KV_BF16) return;
+  __syncthreads();
+  uint8_t* tile = (uint8_t*)a.c.k + (t.head + t.base) * D;
+  for (int i = threadIdx.x; i < 2 * D; i += 256) {  // 16 dims of the slot of tile row i % 32
+    const int j = kv_slot_of_row(i & 31);
+    if (j >= t.lo && j < t.hi) reinterpret_cast<uint4*>(tile)[i] = reinterpret_cast<const uint4*>(lds)[i];
   }
 }
-
-constexpr int KV_DMAX = 128;
 
 // v has no rotation: pieces of 16 dims (V = 8) or of 2, of one token each
 template <int V>
 __device__ void append_v(const KvAppendArgs& a, int vb, char* lds) {
-  const int D = a.c.D, tiles = (a.S + 31) / 32 + 1;  // a row's new slots touch this many tiles at most
-  const int b = vb / (tiles * a.c.n_kv), h = vb / tiles % a.c.n_kv;
-  const int start = a.start[b], n = row_count(a.counts, b, a.S);
-  if (start < 0 && start + (int64_t)n <= 0) return;
-  const int64_t base = ((int64_t)(start >> 5) + vb % tiles) * 32;  // the tile's first slot
-  if (base < 0 || base >= a.c.slots || base >= (int64_t)start + n) return;
-  const int lo = (int)max((int64_t)0, start - base), hi = (int)min((int64_t)32, start + (int64_t)n - base);
-  const size_t head = ((size_t)b * a.c.n_kv + h) * a.c.slots;
-  const int pt = D / (2 * V);
+  KvTile kt;
+  if (!kv_tile(a, vb, &kt)) return;
+  const int D = a.c.D, b = kt.b, h = kt.h, start = kt.start, lo = kt.lo, hi = kt.hi, pt = D / (2 * V);
+  const int64_t base = kt.base;
+  const size_t head = kt.head;
   if (a.c.type == KV_BF16) {
     bf16_t(*t)[KV_DMAX + 8] = reinterpret_cast<bf16_t(*)[KV_DMAX + 8]>(lds);
     for (int i = threadIdx.x; i < 32 * pt; i += 256) {
@@ -385,11 +404,11 @@ __device__ void append_v(const KvAppendArgs& a, int vb, char* lds) {
 }
 
 template <int V>
-__global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a, int nq, int nk, int hq, int hk) {
+__global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a, int nq, int nk, int hq) {
   __shared__ __attribute__((aligned(16))) char lds[32 * (KV_DMAX + 8) * 2];
   const int blk = blockIdx.x;
   if (blk < nq) append_q<V>(a, blk, hq);
-  else if (blk < nq + nk) append_k<V>(a, blk - nq, hk);
+  else if (blk < nq + nk) append_k<V>(a, blk - nq, lds);
   else append_v<V>(a, blk - nq - nk, lds);
 }
 
@@ -408,15 +427,11 @@ hipError_t kv_append(const KvAppendArgs& a, hipStream_t s) {
     while (hq < a.H && M * ((a.H + hq - 1) / hq) > 4096) hq += tpw;
     nq = (M * ((a.H + hq - 1) / hq) + 3) / 4;
   }
-  const int64_t groups = (int64_t)a.B * ((a.S + tpw - 1) / tpw);
-  int hk = 1;
-  while (hk < a.c.n_kv && groups * ((a.c.n_kv + hk - 1) / hk) > 4096) ++hk;
-  const int64_t nk = (groups * ((a.c.n_kv + hk - 1) / hk) + 3) / 4;
-  const int64_t nv = (int64_t)a.B * a.c.n_kv * ((a.S + 31) / 32 + 1);
-  if (nq + nk + nv > INT_MAX) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)(nq + nk + nv));
-  if (v8) hipLaunchKernelGGL(kv_append_kernel<8>, grid, dim3(256), 0, s, a, (int)nq, (int)nk, hq, hk);
-  else hipLaunchKernelGGL(kv_append_kernel<1>, grid, dim3(256), 0, s, a, (int)nq, (int)nk, hq, hk);
+  const int64_t nk = (int64_t)a.B * a.c.n_kv * ((a.S + 31) / 32 + 1);
+  if (nq + 2 * nk > INT_MAX) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)(nq + 2 * nk));
+  if (v8) hipLaunchKernelGGL(kv_append_kernel<8>, grid, dim3(256), 0, s, a, (int)nq, (int)nk, hq);
+  else hipLaunchKernelGGL(kv_append_kernel<1>, grid, dim3(256), 0, s, a, (int)nq, (int)nk, hq);
   return hipGetLastError();
 }
 
@@ -496,68 +511,95 @@ hipError_t kv_read(const KvReadArgs& a, hipStream_t s) {
 
 // ---------------------------------------------------------------------------
 // Compaction: slot start + i <- slot start + path[i], i < took.  A block owns the K or the V of one
-// (row, kv head): it gathers every source into LDS before it writes any slot, so paths may overlap
-// their destinations in any order.  An entry whose source or destination is no slot is left out.
+// (row, kv head) and reads every source before it writes any slot, so paths may overlap their destinations
+// in any order.  An entry whose source or destination is no slot is left out.  K moves in 16-byte pieces.
+// V has its slots side by side, so the window of slots that a path can touch goes through LDS in 16-byte
+// pieces (a piece at an edge writes the slots beside the window back as they were): byte by byte, 64 rows
+// of 64 tokens took 14.5 us.
+constexpr int KV_WIN = KV_PATH_MAX + 32;  // slots of the window: whole tiles (8-bit), or pieces of 8 (bf16)
 __global__ __launch_bounds__(256) void kv_compact_kernel(KvCompactArgs a) {
-  __shared__ __attribute__((aligned(16))) uint8_t rows[KV_PATH_MAX * KV_DMAX * 2];
-  __shared__ float sc[KV_PATH_MAX];
-  const int D = a.c.D, unit = blockIdx.x >> 1, isv = blockIdx.x & 1;
+  __shared__ __attribute__((aligned(16))) uint8_t win[KV_DMAX * (KV_PATH_MAX + 8) * 2];
+  __shared__ int from[KV_PATH_MAX];  // the slot that entry i takes, -1: none
+  const int D = a.c.D, unit = blockIdx.x >> 1, isv = blockIdx.x & 1, tid = threadIdx.x;
   const int b = unit / a.c.n_kv;
-  const int start = a.start[b], n = min(max(a.took[b], 0), a.P);
-  const size_t head = (size_t)unit * a.c.slots;  // unit = b * n_kv + h
-  const int* path = a.path + (size_t)b * a.P;
-  auto src = [&](int i) -> int {  // the slot that entry i takes, -1: none
-    const int p = path[i];
-    if (p < 0 || p >= KV_PATH_MAX) return -1;
-    const int64_t from = (int64_t)start + p, to = (int64_t)start + i;
-    return from < 0 || from >= a.c.slots || to < 0 || to >= a.c.slots ? -1 : (int)from;
-  };
+  const int start = a.start[b], n = min(max(a.took[b], 0), a.P), slots = a.c.slots;
+  if (n == 0) return;
+  const size_t head = (size_t)unit * slots;  // unit = b * n_kv + h
   const bool bf = a.c.type == KV_BF16;
   float* scales = isv ? a.c.vs : a.c.ks;
-  if (!bf)
-    for (int i = threadIdx.x; i < n; i += 256) {
-      const int f = src(i);
-      sc[i] = f < 0 ? 0.f : scales[head + f];
-    }
-  if (!isv) {  // K: 16-byte pieces, 8 or 16 values each
-    const int per = bf ? 8 : 16, np = D / per;
-    uint4* l = reinterpret_cast<uint4*>(rows);
-    uint8_t* k = (uint8_t*)a.c.k;
-    auto at = [&](int slot, int c) -> uint4* {
-      return bf ? reinterpret_cast<uint4*>(k + ((head + slot) * D + c * 8) * 2)
-                : reinterpret_cast<uint4*>(k + (head + (slot & ~31)) * D + kv_k_byte(slot & 31, c * 16));
-    };
-    for (int i = threadIdx.x; i < n * np; i += 256) {
-      const int f = src(i / np);
-      if (f >= 0) l[i] = *at(f, i % np);
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < n * np; i += 256)
-      if (src(i / np) >= 0) *at(start + i / np, i % np) = l[i];
-  } else if (bf) {
-    bf16_t* l = reinterpret_cast<bf16_t*>(rows);
-    bf16_t* v = (bf16_t*)a.c.v + head * D;
-    for (int i = threadIdx.x; i < n * D; i += 256) {
-      const int f = src(i / D);
-      if (f >= 0) l[i] = v[(size_t)(i % D) * a.c.slots + f];
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < n * D; i += 256)
-      if (src(i / D) >= 0) v[(size_t)(i % D) * a.c.slots + start + i / D] = l[i];
-  } else {
-    uint8_t* v = (uint8_t*)a.c.v;
-    auto at = [&](int slot, int d) -> uint8_t* { return v + (head + (slot & ~31)) * D + kv_v_byte(slot & 31, d); };
-    for (int i = threadIdx.x; i < n * D; i += 256) {
-      const int f = src(i / D);
-      if (f >= 0) rows[i] = *at(f, i % D);
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < n * D; i += 256)
-      if (src(i / D) >= 0) *at(start + i / D, i % D) = rows[i];
+  float sc = 0.f;
+  if (tid < n) {
+    const int p = a.path[(size_t)b * a.P + tid];
+    const int64_t f = (int64_t)start + p, t = (int64_t)start + tid;
+    const bool ok = p >= 0 && p < KV_PATH_MAX && f >= 0 && f < slots && t >= 0 && t < slots;
+    from[tid] = ok ? (int)f : -1;
+    if (ok && !bf) sc = scales[head + f];
   }
-  if (!bf)
-    for (int i = threadIdx.x; i < n; i += 256)
-      if (src(i) >= 0) scales[head + start + i] = sc[i];
+  __syncthreads();
+  if (!isv) {
+    const int np = bf ? D / 8 : D / 16;  // pieces a slot
+    uint8_t* k = (uint8_t*)a.c.k;
+    auto at = [&](int slot, int c) -> u32x4* {
+      return bf ? reinterpret_cast<u32x4*>(k + ((head + slot) * D + c * 8) * 2)
+                : reinterpret_cast<u32x4*>(k + (head + (slot & ~31)) * D + kv_k_byte(slot & 31, c * 16));
+    };
+    u32x4 x[4];  // KV_PATH_MAX * KV_DMAX / 8 / 256
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = tid + 256 * j, e = i / np;
+      if (e < n && from[e] >= 0) x[j] = *at(from[e], i - e * np);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = tid + 256 * j, e = i / np;
+      if (e < n && from[e] >= 0) *at(start + e, i - e * np) = x[j];
+    }
+  } else if (bf) {
+    // [D][KV_PATH_MAX + 8] values from slot `lo` on
+    constexpr int NW = KV_PATH_MAX + 8;
+    const int lo = max(start, 0) & ~7;
+    bf16_t* w = reinterpret_cast<bf16_t*>(win);
+    bf16_t* v = (bf16_t*)a.c.v + head * D + lo;
+    for (int i = tid; i < D * (NW / 8); i += 256) {
+      const int d = i / (NW / 8), c = i % (NW / 8) * 8;
+      if (lo + c < slots) *reinterpret_cast<uint4*>(w + d * NW + c) = *reinterpret_cast<const uint4*>(v + (size_t)d * slots + c);
+    }
+    __syncthreads();
+    for (int i = tid; i < D * (NW / 8); i += 256) {
+      const int d = i / (NW / 8), c = i % (NW / 8) * 8;
+      if (lo + c >= slots || lo + c >= (int64_t)start + n) continue;
+      uint32_t o[4];
+#pragma unroll
+      for (int y = 0; y < 8; ++y) {
+        const int e = lo + c + y - start;
+        const int f = e >= 0 && e < n && from[e] >= 0 ? from[e] - lo : c + y;
+        const uint32_t z = w[d * NW + f];
+        o[y >> 1] = y & 1 ? o[y >> 1] | z << 16 : z;
+      }
+      *reinterpret_cast<uint4*>(v + (size_t)d * slots + c) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+  } else {
+    // the window's tiles as they lie
+    const int t0 = max(start, 0) & ~31, nt = min(KV_WIN, slots - t0) >> 5;
+    uint8_t* v = (uint8_t*)a.c.v + (head + t0) * D;
+    for (int i = tid; i < nt * 2 * D; i += 256) reinterpret_cast<uint4*>(win)[i] = reinterpret_cast<const uint4*>(v)[i];
+    __syncthreads();
+    for (int i = tid; i < nt * 2 * D; i += 256) {
+      const int tile = i / (2 * D), j = i - tile * 2 * D;  // 16 bytes: slots 16 u + 8 h + y of one dim
+      if (t0 + tile * 32 >= (int64_t)start + n) break;
+      const int d = (j >> 6) * 32 + (j & 31), hh = (j >> 5) & 1;
+      uint32_t o[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int y = 0; y < 16; ++y) {
+        const int s = tile * 32 + (y >> 3) * 16 + hh * 8 + (y & 7), e = t0 + s - start;
+        const int f = e >= 0 && e < n && from[e] >= 0 ? from[e] - t0 : s;
+        o[y >> 2] |= (uint32_t)win[(f >> 5) * 32 * D + kv_v_byte(f & 31, d)] << (8 * (y & 3));
+      }
+      reinterpret_cast<uint4*>(v)[i] = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+  }
+  if (!bf && tid < n && from[tid] >= 0) scales[head + start + tid] = sc;
 }
 
 hipError_t kv_compact(const KvCompactArgs& a, hipStream_t s) {

@@ -97,28 +97,30 @@ class Rope:
         self.turns = turns.to(self.device).contiguous()
         self._c = N.MttsRope(self.turns.data_ptr(), self.rotary_dim, int(self.interleaved), self.factor)
         self._ref = ctypes.addressof(self._c)
-        self._fn = N.load().mtts_k_rope
+        self._fn, self._index = N.load().mtts_k_rope, self.device.index
 
     def apply(self, x: torch.Tensor, positions: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """x bf16 [M, H, head_dim] (any strides between tokens and heads) at int32 positions [M];
         `out` may be x itself."""
-        _need(x.dim() == 3 and x.dtype == torch.bfloat16 and x.shape[2] == self.head_dim and x.device == self.device,
-              "x is bf16 [tokens, heads, head_dim] on the frequencies' device")
+        if x.dim() != 3 or x.dtype is not torch.bfloat16 or x.shape[2] != self.head_dim or x.device != self.device:
+            raise ValueError("x is bf16 [tokens, heads, head_dim] on the frequencies' device")
         M, H, D = x.shape
         xs = x.stride()
         if out is None:
             out, ys = torch.empty((M, H, D), dtype=torch.bfloat16, device=self.device), (H * D, D, 1)
+        elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+            raise ValueError("out is like x")
         else:
-            _need(out.shape == x.shape and out.dtype == x.dtype and out.device == x.device, "out is like x")
             ys = out.stride()
-        _need(xs[2] == 1 and ys[2] == 1, "a head's dims lie side by side")
-        _call("rope", self._fn, self.device.index, x.data_ptr(), xs[0], xs[1], out.data_ptr(), ys[0], ys[1],
+        if xs[2] != 1 or ys[2] != 1:
+            raise ValueError("a head's dims lie side by side")
+        _call("rope", self._fn, self._index, x.data_ptr(), xs[0], xs[1], out.data_ptr(), ys[0], ys[1],
               _i32(positions, (M,), self.device, "positions"), M, H, D, self._ref)
         return out
 
 
 def _i32(t, shape, device, what):
-    if t.dtype != torch.int32 or t.shape != shape or t.device != device or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{what}: contiguous int32 {list(shape)} on {device}")
     return t.data_ptr()
 
@@ -168,6 +170,7 @@ class KVCache:
                                 None if self.v_scale is None else self.v_scale.data_ptr(), DTYPES[dtype], rows, n_kv,
                                 head_dim, self.slots)
         self._ref = ctypes.addressof(self._c)
+        self._index = self.device.index
         L = N.load()
         self._f_append, self._f_read, self._f_compact = L.mtts_k_kv_append, L.mtts_k_kv_read, L.mtts_k_kv_compact
         self._f_attn, self._f_ws = L.mtts_k_attn_kv, L.mtts_k_attn_kv_ws_bytes
@@ -176,7 +179,8 @@ class KVCache:
         return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale) if t is not None)
 
     def _start(self, start, B):
-        _need(B <= self.rows, f"{B} rows for a cache of {self.rows}")
+        if B > self.rows:
+            raise ValueError(f"{B} rows for a cache of {self.rows}")
         return _i32(start, (B,), self.device, "start")
 
     def _counts(self, counts, B):
@@ -185,16 +189,19 @@ class KVCache:
     def _norm(self, w, what):
         if w is None:
             return None
-        _need(w.dtype == torch.bfloat16 and w.shape == (self.head_dim,) and w.is_contiguous() and w.device == self.device,
-              f"{what}: bf16 [head_dim]")
+        if w.dtype is not torch.bfloat16 or w.shape != (self.head_dim,) or not w.is_contiguous() or w.device != self.device:
+            raise ValueError(f"{what}: bf16 [head_dim]")
         return w.data_ptr()
 
-    def _append(self, q, k, v, out, n_heads, ld, B, S, start, rope, positions, counts, q_norm, k_norm, eps):
+    def _append(self, q, k, v, out, n_heads, ldq, ldk, ldv, B, S, start, rope, positions, counts, q_norm, k_norm, eps):
+        r = None
         if rope is not None:
-            _need(rope.head_dim == self.head_dim and rope.device == self.device, "rope is of another head or device")
-        _call("append", self._f_append, self.device.index, self._ref, q, ld[0], k, ld[1], v, ld[2],
+            if rope.head_dim != self.head_dim or rope.device != self.device:
+                raise ValueError("rope is of another head or device")
+            r = rope._ref
+        _call("append", self._f_append, self._index, self._ref, q, ldq, k, ldk, v, ldv,
               None if out is None else out.data_ptr(), n_heads * self.head_dim, n_heads, self._norm(q_norm, "q_norm"),
-              self._norm(k_norm, "k_norm"), eps, None if rope is None else rope._ref,
+              self._norm(k_norm, "k_norm"), eps, r,
               None if positions is None else _i32(positions, (B, S), self.device, "positions"), self._start(start, B),
               self._counts(counts, B), B, S)
 
@@ -207,20 +214,23 @@ class KVCache:
         returns q [B, S, n_heads, head_dim].  Rows behind counts[b] (int32 [B]; None: S) store nothing;
         their q is zero, or what `out` held."""
         D = self.head_dim
-        _need(qkv.dim() == 3 and qkv.dtype == torch.bfloat16 and qkv.device == self.device and
-              n_heads > 0 and qkv.shape[2] == (n_heads + 2 * self.n_kv) * D, "qkv: bf16 [B, S, (n_heads + 2 n_kv) * head_dim]")
+        if (qkv.dim() != 3 or qkv.dtype is not torch.bfloat16 or qkv.device != self.device or n_heads < 1 or
+                qkv.shape[2] != (n_heads + 2 * self.n_kv) * D):
+            raise ValueError("qkv: bf16 [B, S, (n_heads + 2 n_kv) * head_dim]")
         B, S, _ = qkv.shape
-        ld = qkv.stride(1) if S > 1 else qkv.stride(0)
-        _need(qkv.stride(2) == 1 and (B <= 1 or S <= 1 or qkv.stride(0) == S * qkv.stride(1)), "qkv: rows one stride apart")
+        s0, s1, s2 = qkv.stride()
+        if s2 != 1 or (B > 1 and S > 1 and s0 != S * s1):
+            raise ValueError("qkv: rows one stride apart")
+        ld = s1 if S > 1 else s0
         if out is None:
             out = (torch.empty if counts is None else torch.zeros)((B, S, n_heads, D), dtype=torch.bfloat16,
                                                                   device=self.device)
-        else:
-            _need(out.shape == (B, S, n_heads, D) and out.dtype == torch.bfloat16 and out.is_contiguous() and
-                  out.device == self.device, "out: contiguous bf16 [B, S, n_heads, head_dim]")
+        elif (out.shape != (B, S, n_heads, D) or out.dtype is not torch.bfloat16 or not out.is_contiguous() or
+              out.device != self.device):
+            raise ValueError("out: contiguous bf16 [B, S, n_heads, head_dim]")
         p = qkv.data_ptr()
-        self._append(p, p + 2 * n_heads * D, p + 2 * (n_heads + self.n_kv) * D, out, n_heads, (ld, ld, ld), B, S, start,
-                     rope, positions, counts, q_norm, k_norm, eps)
+        self._append(p, p + 2 * n_heads * D, p + 2 * (n_heads + self.n_kv) * D, out, n_heads, ld, ld, ld, B, S, start, rope,
+                     positions, counts, q_norm, k_norm, eps)
         return out
 
     def write(self, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor, rope: Optional[Rope] = None,
@@ -229,34 +239,36 @@ class KVCache:
         lds = []
         B, S = k.shape[:2]
         for t in (k, v):
-            _need(t.dim() == 4 and t.dtype == torch.bfloat16 and t.device == self.device and
-                  t.shape == (B, S, self.n_kv, self.head_dim), "k, v: bf16 [B, S, n_kv, head_dim]")
-            ld = t.stride(1) if S > 1 else t.stride(0)
-            _need(t.stride(3) == 1 and (self.n_kv == 1 or t.stride(2) == self.head_dim) and
-                  (B <= 1 or S <= 1 or t.stride(0) == S * t.stride(1)), "k, v: heads side by side, rows one stride apart")
-            lds.append(ld)
-        self._append(None, k.data_ptr(), v.data_ptr(), None, 0, (0, *lds), B, S, start, rope, positions, counts, None, None,
-                     0.0)
+            if t.dim() != 4 or t.dtype is not torch.bfloat16 or t.device != self.device or \
+                    t.shape != (B, S, self.n_kv, self.head_dim):
+                raise ValueError("k, v: bf16 [B, S, n_kv, head_dim]")
+            s0, s1, s2, s3 = t.stride()
+            if s3 != 1 or (self.n_kv > 1 and s2 != self.head_dim) or (B > 1 and S > 1 and s0 != S * s1):
+                raise ValueError("k, v: heads side by side, rows one stride apart")
+            lds.append(s1 if S > 1 else s0)
+        self._append(None, k.data_ptr(), v.data_ptr(), None, 0, 0, lds[0], lds[1], B, S, start, rope, positions, counts, None,
+                     None, 0.0)
 
     def read(self, n: int, start: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None,
              rows: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """Slots start[b] (None: 0) .. + n - 1 of the first `rows` rows (default: start's, or all) as bf16
         (k, v), each [rows, n_kv, n, head_dim]; rows behind counts[b] and slots past the end are zeros."""
         B = rows if rows is not None else self.rows if start is None else start.shape[0]
-        _need(n >= 0 and B >= 0, "read: sizes")
-        _need(B <= self.rows, f"{B} rows for a cache of {self.rows}")
+        if n < 0 or not 0 <= B <= self.rows:
+            raise ValueError(f"read: {n} slots of {B} rows, of a cache of {self.rows}")
         k = torch.empty((B, self.n_kv, n, self.head_dim), dtype=torch.bfloat16, device=self.device)
         v = torch.empty_like(k)
-        _call("read", self._f_read, self.device.index, self._ref, k.data_ptr(), v.data_ptr(),
+        _call("read", self._f_read, self._index, self._ref, k.data_ptr(), v.data_ptr(),
               None if start is None else self._start(start, B), self._counts(counts, B), B, n)
         return k, v
 
     def compact(self, start: torch.Tensor, path: torch.Tensor, accepted: torch.Tensor) -> None:
         """Keeps the accepted path of a drafted tree: slot start[b] + i takes what slot start[b] +
         path[b, i] holds, for i < accepted[b] (path int32 [B, P], P <= 64; accepted int32 [B])."""
-        _need(path.dim() == 2, "path: int32 [B, P]")
+        if path.dim() != 2:
+            raise ValueError("path: int32 [B, P]")
         B, P = path.shape
-        _call("compact", self._f_compact, self.device.index, self._ref, self._start(start, B),
+        _call("compact", self._f_compact, self._index, self._ref, self._start(start, B),
               _i32(path, (B, P), self.device, "path"), _i32(accepted, (B,), self.device, "accepted"), B, P)
 
     def attend(self, q: torch.Tensor, start: torch.Tensor, tree: Optional[torch.Tensor] = None,
@@ -267,30 +279,34 @@ class KVCache:
         attend) keeps and the new tokens that tree (int64 [B, T], `tree_masks`; None: a chain) shows.
         A token that sees nothing gets zeros; rows behind counts[b] are zero, or what `out` held.
         max_len: an upper bound of `start` known to the caller, for the shape of the launch only."""
-        _need(q.dim() == 4 and q.dtype == torch.bfloat16 and q.shape[3] == self.head_dim and q.device == self.device,
-              "q: bf16 [B, T, n_heads, head_dim]")
+        if q.dim() != 4 or q.dtype is not torch.bfloat16 or q.shape[3] != self.head_dim or q.device != self.device:
+            raise ValueError("q: bf16 [B, T, n_heads, head_dim]")
         B, T, H, D = q.shape
-        ldq = q.stride(1) if T > 1 else q.stride(0)
-        _need(q.stride(3) == 1 and (H == 1 or q.stride(2) == D) and (B <= 1 or T <= 1 or q.stride(0) == T * q.stride(1)),
-              "q: heads side by side, rows one stride apart")
+        s0, s1, s2, s3 = q.stride()
+        if s3 != 1 or (H > 1 and s2 != D) or (B > 1 and T > 1 and s0 != T * s1):
+            raise ValueError("q: heads side by side, rows one stride apart")
+        tp = mp = None
         if tree is not None:
-            _need(tree.dtype == torch.int64 and tree.shape == (B, T) and tree.is_contiguous() and
-                  tree.device == self.device, "tree: contiguous int64 [B, T]")
+            if tree.dtype is not torch.int64 or tree.shape != (B, T) or not tree.is_contiguous() or tree.device != self.device:
+                raise ValueError("tree: contiguous int64 [B, T]")
+            tp = tree.data_ptr()
         if mask is not None:
-            _need(mask.dtype in (torch.uint8, torch.bool) and mask.shape == (B, self.slots) and mask.is_contiguous() and
-                  mask.device == self.device, f"mask: contiguous uint8 [B, {self.slots}]")
+            if mask.dtype not in (torch.uint8, torch.bool) or mask.shape != (B, self.slots) or not mask.is_contiguous() or \
+                    mask.device != self.device:
+                raise ValueError(f"mask: contiguous uint8 [B, {self.slots}]")
+            mp = mask.data_ptr()
         if out is None:
             out = (torch.empty if counts is None else torch.zeros)((B, T, H, D), dtype=torch.bfloat16, device=self.device)
-        else:
-            _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous() and out.device == self.device,
-                  "out: contiguous, like q")
-        _need(scale is None or scale > 0, "scale > 0")
+        elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != self.device:
+            raise ValueError("out: contiguous, like q")
+        if scale is None:
+            scale = 0.0
+        elif not scale > 0:
+            raise ValueError("scale > 0")
         n = 0 if max_len is None else max(1, int(max_len))
         need = self._f_ws(B, T, H, self.n_kv, D, self.slots, n)
         # (scratch of this call alone, from torch's allocator: in order on this stream, a graph's own in a capture)
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        _call("attend", self._f_attn, self.device.index, self._ref, q.data_ptr(), ldq, out.data_ptr(), H * D, H,
-              self._start(start, B), self._counts(counts, B), None if tree is None else tree.data_ptr(),
-              None if mask is None else mask.data_ptr(), B, T, 0.0 if scale is None else scale, n,
-              None if ws is None else ws.data_ptr())
+        _call("attend", self._f_attn, self._index, self._ref, q.data_ptr(), s1 if T > 1 else s0, out.data_ptr(), H * D, H,
+              self._start(start, B), self._counts(counts, B), tp, mp, B, T, scale, n, None if ws is None else ws.data_ptr())
         return out
