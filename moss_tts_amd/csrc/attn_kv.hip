@@ -123,6 +123,18 @@ struct Segments {
     return true;
   }
 };
+// f of each segment of block x.  Unsplit launches (SPLIT false) have a kernel of their own: with the sharing
+// out in it too it is twice the code, whose fetching a short call waits for (one token over 389 bf16 slots
+// 10.3 us and not 8), and the loop over 32 rows of 4,000 slots took 94 us and not 81.
+template <bool SPLIT, int SEG, class F>
+__device__ __forceinline__ void for_segments(const AttnKvArgs& a, int NS, int least, int x, bool head, F&& f) {
+  if constexpr (SPLIT) {
+    Segments<SEG> it(a, NS, least, x, head);
+    for (Seg sg; it.next(sg);) f(sg);
+  } else {
+    f(Seg{x, 0, INT_MAX, -1, row_len(a, x)});
+  }
+}
 // floats at the head of the workspace
 __host__ __device__ __forceinline__ size_t head_floats(int B) { return ((size_t)2 * B + 63) / 64 * 64; }
 
@@ -506,7 +518,7 @@ struct Stage {
 // Up to 32 rows a KV head (a decode step, a small tree): bound by the cache's bytes.  The NW waves of a
 // block take tiles in turn, loaded one tile ahead, with no barrier in the loop, and merge once at the
 // end.  8-bit fragments go from memory straight into registers, bf16 ones through LDS of the wave's own.
-template <int KT, int D, int NW>
+template <int KT, int D, int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, 2) void attn_kv_keys(AttnKvArgs a, int NS, int least, uint32_t rG) {
   constexpr bool Q8 = KT != KV_BF16;
   constexpr int NF = D / 32;
@@ -536,10 +548,10 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_kv_keys(AttnKvArgs a, int NS,
   auto load_k = [&](int t) {
     const char* p = kb + (size_t)t * (32 * D);
 #pragma unroll
-      for (int j = 0; j < NF; ++j) kf[j] = *reinterpret_cast<const u32x4*>(p + (uint32_t)(j * 1024 + lane * 16));
-      ksn = (a.c.ks + head + t * 32)[sl];
-      vsn = (a.c.vs + head + t * 32)[sl];
-    };
+    for (int j = 0; j < NF; ++j) kf[j] = *reinterpret_cast<const u32x4*>(p + (uint32_t)(j * 1024 + lane * 16));
+    ksn = (a.c.ks + head + t * 32)[sl];
+    vsn = (a.c.vs + head + t * 32)[sl];
+  };
   auto load_v = [&](int t) {
     const char* p = vb + (size_t)t * (32 * D);
 #pragma unroll
@@ -554,21 +566,19 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_kv_keys(AttnKvArgs a, int NS,
       sv.load_v(vb, slots, t, 0, lane);
     }
   };
-  // an unsplit row's first tiles are known before its length is (and there, whatever that turns out to be;
-  // 8-bit: bf16 has no registers left for it)
-  if (Q8 && least == 0) {
+  // an unsplit row's first tiles are known before its length is (and there, whatever that turns out to be)
+  if constexpr (!SPLIT) {
     row_at(x);
     load_tile(min(wave, (slots >> 5) - 1));
   }
-  Segments<16> it(a, NS, least, x, hkv == 0 && x == 0);
-  for (Seg sg; it.next(sg);) {
+  for_segments<SPLIT, 16>(a, NS, least, x, hkv == 0 && x == 0, [&](const Seg& sg) {
     const int b = sg.b;
     const RowLen len = sg.len;
     const int R = len.n * G;
-    if (R == 0) continue;
+    if (R == 0) return;
     const int t1 = min(sg.t1, (len.nk + 31) >> 5);
     int tile = sg.t0 + wave;
-    if (!Q8 || least) {
+    if constexpr (SPLIT) {
       row_at(b);
       if (tile < t1) load_tile(tile);
     }
@@ -657,7 +667,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_kv_keys(AttnKvArgs a, int NS,
               make_float4(st.o[t][i], st.o[t][i + 1], st.o[t][i + 2], st.o[t][i + 3]);
     }
     __syncthreads();
-    const bool whole = sg.slot < 0;
+    const bool whole = !SPLIT || sg.slot < 0;
     float* po = a.part + head_floats(a.B) + (size_t)(sg.slot * Hkv + hkv) * 32 * (D + 2);
     for (int q = threadIdx.x; q < R * (D / 4); q += 64 * NW) {
       const int r = q / (D / 4), d = q % (D / 4) * 4;
@@ -683,16 +693,15 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_kv_keys(AttnKvArgs a, int NS,
         *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(y.x * sc, y.y * sc), pack2(y.z * sc, y.w * sc));
       }
     }
-    if (least) __syncthreads();  // (the next segment writes LDS)
-  }
+    if constexpr (SPLIT) __syncthreads();  // (the next segment writes LDS)
+  });
 }
 
 // More rows: bound by the arithmetic on the scores.  The W waves of a block, 32 rows each, go through the
 // same tiles, whose fragments they load, turn into bf16 and put into LDS together, once for all rows, one
 // tile ahead of the products (two LDS buffers, one barrier a tile).
 template <int KT, int D, int W>
-__global__ __launch_bounds__(64 * W, 2) void attn_kv_rows(AttnKvArgs a, int NS,
-                                                                                              int least, int RB) {
+__global__ __launch_bounds__(64 * W, 2) void attn_kv_rows(AttnKvArgs a, int NS, int least, int RB) {
   constexpr bool Q8 = KT != KV_BF16;
   constexpr int DT = D / 32, rows = 32 * W;
   constexpr int TT = W == 2 ? 1 : 2;  // tiles a turn (LDS for 4 blocks of 2 waves, or 2 of 4, or 1 of 8)
@@ -953,26 +962,34 @@ size_t attn_kv_ws_bytes(int B, int T, int Hq, int n_kv, int D, int slots, int ma
   return (head_floats(B) + (size_t)2 * p.NS * n_kv * p.RB * 32 * std::max(1, p.W) * (D + 2)) * sizeof(float);
 }
 
-template <int KT, int D>
-static hipError_t launch(const AttnKvArgs& a, const AkvPlan& p, hipStream_t s) {
-  const int64_t grid = ((int64_t)p.NS * a.c.n_kv + 7) / 8 * 8 * p.RB;
-  const int GS = p.NS > 4 * a.B ? 8 : 1;  // (rows of many partials: they are read at once, not one after the other)
-  const int64_t join = ((int64_t)a.B * a.T * a.Hq * (D / 4) * GS + 255) / 256;
-  if (grid > INT_MAX || join > INT_MAX || (p.W == 0 && p.NS > 65535)) return hipErrorInvalidValue;
+template <int KT, int D, bool SPLIT>
+static void launch_form(const AttnKvArgs& a, const AkvPlan& p, int64_t grid, hipStream_t s) {
   const dim3 g((unsigned)grid);
   switch (p.W) {
     case 0: {
       const uint32_t G = a.Hq / a.c.n_kv, rG = (65536 + G - 1) / G;
-      hipLaunchKernelGGL((attn_kv_keys<KT, D, 8>), dim3(a.c.n_kv, p.NS), dim3(512), 0, s, a, p.NS, p.least, rG);
+      hipLaunchKernelGGL((attn_kv_keys<KT, D, 8, SPLIT>), dim3(a.c.n_kv, p.NS), dim3(512), 0, s, a, p.NS, p.least, rG);
       break;
     }
     case 2: hipLaunchKernelGGL((attn_kv_rows<KT, D, 2>), g, dim3(128), 0, s, a, p.NS, p.least, p.RB); break;
     case 4: hipLaunchKernelGGL((attn_kv_rows<KT, D, 4>), g, dim3(256), 0, s, a, p.NS, p.least, p.RB); break;
     default: hipLaunchKernelGGL((attn_kv_rows<KT, D, 8>), g, dim3(512), 0, s, a, p.NS, p.least, p.RB);
   }
-  if (p.least && GS == 8)
+}
+template <int KT, int D>
+static hipError_t launch(const AttnKvArgs& a, const AkvPlan& p, hipStream_t s) {
+  const int64_t grid = ((int64_t)p.NS * a.c.n_kv + 7) / 8 * 8 * p.RB;
+  const int GS = p.NS > 4 * a.B ? 8 : 1;  // (rows of many partials: they are read at once, not one after the other)
+  const int64_t join = ((int64_t)a.B * a.T * a.Hq * (D / 4) * GS + 255) / 256;
+  if (grid > INT_MAX || join > INT_MAX || (p.W == 0 && p.NS > 65535)) return hipErrorInvalidValue;
+  if (!p.least) {
+    launch_form<KT, D, false>(a, p, grid, s);
+    return hipGetLastError();
+  }
+  launch_form<KT, D, true>(a, p, grid, s);
+  if (GS == 8)
     hipLaunchKernelGGL((attn_kv_join<D, 8>), dim3((unsigned)join), dim3(256), 0, s, a, p.RB, 32 * std::max(1, p.W));
-  else if (p.least)
+  else
     hipLaunchKernelGGL((attn_kv_join<D, 1>), dim3((unsigned)join), dim3(256), 0, s, a, p.RB, 32 * std::max(1, p.W));
   return hipGetLastError();
 }
