@@ -316,7 +316,7 @@ int mtts_k_fill_uniform(uint16_t* dst, size_t n, uint64_t seed, uint64_t tensor_
 typedef struct mtts_kv_cache {
   void *k, *v;              /* mtts_kv_bytes each, 16-byte aligned */
   float *k_scale, *v_scale; /* [rows][n_kv][slots]; unused for MTTS_KV_BF16 */
-  int type, rows, n_kv, head_dim, slots; /* head_dim 32 / 64 / 128; slots a multiple of 32 */
+  int type, rows, n_kv, head_dim, slots; /* head_dim 32 / 64 / 128; slots a multiple of 32, below 2^25 */
 } mtts_kv_cache;
 /* bytes of k (and of v): the scales are rows * n_kv * slots floats each */
 size_t mtts_kv_bytes(int type, int rows, int n_kv, int head_dim, int slots);
@@ -343,8 +343,8 @@ typedef struct mtts_rope_scaling {
 } mtts_rope_scaling;
 /* host: turns_host[rotary_dim / 2] and the factor for a base and a scaling (NULL: none) */
 int mtts_rope_turns(double theta, int rotary_dim, const mtts_rope_scaling* scaling, double* turns_host, float* factor);
-/* y = rotated x: M tokens of H heads, ld* elements between tokens, hs* between heads; y may be x (with
- * its strides).  pos_dev int32 [M].  head_dim even. */
+/* y = rotated x: M tokens of H heads, ld* elements between tokens, hs* between heads (x's may
+ * be 0); y is x with its strides, or shares no head with it.  pos_dev int32 [M].  head_dim even. */
 int mtts_k_rope(const uint16_t* x, size_t ldx, size_t hsx, uint16_t* y, size_t ldy, size_t hsy, const int32_t* pos_dev,
                 int M, int H, int head_dim, const mtts_rope* rope, void* stream);
 
@@ -376,7 +376,7 @@ int mtts_k_kv_compact(const mtts_kv_cache* cache, const int32_t* start_dev, cons
  * at + (b * T + t) * ld, [n_heads][head_dim]; rows behind counts[b] are left as they are.
  * max_len: an upper bound of start the caller knows (<= 0: slots); it sizes the launch, not the result.
  * ws_dev: mtts_k_attn_kv_ws_bytes bytes of scratch (0: NULL is fine), not shared by calls that may run
- * at once; nothing is kept in it. */
+ * at once; nothing is kept in it.  At most 65,535 rows. */
 size_t mtts_k_attn_kv_ws_bytes(int B, int T, int n_heads, int n_kv, int head_dim, int slots, int max_len);
 int mtts_k_attn_kv(const mtts_kv_cache* cache, const uint16_t* q, size_t ldq, uint16_t* out, size_t ldo, int n_heads,
                    const int32_t* start_dev, const int32_t* counts_dev, const uint64_t* tree_dev, const uint8_t* mask_dev,

@@ -25,15 +25,16 @@ namespace mtts {
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
 
-// context, new tokens and visible slots of row b; a row's slots end with the cache
+// context, new tokens and visible slots of row b.  New token u stands at slot start + u, if there is one:
+// behind the cache's end there is none, nor before slot 0 (a negative start leaves no context)
 struct RowLen {
   int start, n, nk;
 };
 __device__ __forceinline__ RowLen row_len(const AttnKvArgs& a, int b) {
   RowLen r;
-  r.start = min(max(a.start[b], 0), a.c.slots);
+  r.start = min(max(a.start[b], -(1 << 30)), a.c.slots);
   r.n = a.counts ? min(max(a.counts[b], 0), a.T) : a.T;
-  r.nk = (int)min((int64_t)r.start + r.n, (int64_t)a.c.slots);
+  r.nk = (int)max((int64_t)0, min((int64_t)r.start + r.n, (int64_t)a.c.slots));
   return r;
 }
 
@@ -44,7 +45,7 @@ __device__ __forceinline__ RowLen row_len(const AttnKvArgs& a, int b) {
 // 2 x if it began before, and the join adds them up in order: the first block and the number of blocks of
 // each row stand at the head of the workspace.  share 0: a block a row, nothing to join.
 // A segment more costs a block about SEG tiles (its loads start anew), so a row counts for SEG more.
-__device__ __forceinline__ int tiles_of(const RowLen& r) { return r.n ? (r.nk + 31) >> 5 : 0; }
+__device__ __forceinline__ int tiles_of(const RowLen& r) { return r.n ? max(1, (r.nk + 31) >> 5) : 0; }
 // sum up to and with this lane: rows of 16 lanes by shifts, then the rows' sums by broadcasts
 __device__ __forceinline__ int wave_iscan(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);

@@ -31,6 +31,13 @@ bool rope_of(const mtts_rope* r, int D, RopeView* v) {
   return true;
 }
 
+// n rows of m pieces of d elements, at strides ld and hs: no two meet (one side's run lies within a stride of
+// the other)
+bool apart(int n, size_t ld, int m, size_t hs, size_t d) {
+  if (n > 1 && m > 1) return (hs >= d && ld >= (m - 1) * hs + d) || (ld >= d && hs >= (n - 1) * ld + d);
+  return (n < 2 || ld >= d) && (m < 2 || hs >= d);
+}
+
 }  // namespace
 
 #define KV_CACHE(c, v)                                            \
@@ -90,7 +97,10 @@ extern "C" int mtts_k_rope(const uint16_t* x, size_t ldx, size_t hsx, uint16_t* 
   RopeArgs a{x, y, ldx, hsx, ldy, hsy, pos, M, H, D, {}};
   if (!x || !y || !pos || !rope || !rope_of(rope, D, &a.r)) return fail(MTTS_E_INVALID, "rope: bad arguments");
   if (x == y && (ldx != ldy || hsx != hsy)) return fail(MTTS_E_INVALID, "rope: in place needs the same strides");
-  if ((H > 1 && (hsx < (size_t)D || hsy < (size_t)D))) return fail(MTTS_E_INVALID, "rope: heads overlap");
+  if (!apart(M, ldy, H, hsy, D)) return fail(MTTS_E_INVALID, "rope: the output's heads overlap");
+  // an output inside the input's extent, but not between its heads, would be read after it was written
+  const uintptr_t x0 = (uintptr_t)x, y0 = (uintptr_t)y, gap = x0 < y0 ? y0 - x0 : x0 - y0;
+  if (x != y && gap < 2 * (size_t)D) return fail(MTTS_E_INVALID, "rope: the output overlaps the input");
   HIPCHK(rope_apply(a, (hipStream_t)stream));
   return 0;
 }
@@ -104,6 +114,7 @@ extern "C" int mtts_k_kv_append(const mtts_kv_cache* cache, const uint16_t* q, s
   if (B < 0 || B > c.rows || S < 0) return fail(MTTS_E_INVALID, "append: more rows than the cache has");
   if (B == 0 || S == 0) return 0;
   if (!k || !v || !start || (q && (!q_out || n_heads < 1))) return fail(MTTS_E_INVALID, "append: missing arguments");
+  if (q && (int64_t)B * S > 1 && ldqo < (size_t)n_heads * c.D) return fail(MTTS_E_INVALID, "append: rows of q_out overlap");
   KvAppendArgs a{c, q, k, v, ldq, ldk, ldv, q_out, ldqo, n_heads, qn, kn, eps, {}, pos, start, counts, B, S};
   if (!rope_of(rope, c.D, &a.r)) return fail(MTTS_E_INVALID, "append: rotary dim is even and at most the head's");
   HIPCHK(kv_append(a, (hipStream_t)stream));
@@ -148,6 +159,7 @@ extern "C" int mtts_k_attn_kv(const mtts_kv_cache* cache, const uint16_t* q, siz
   if (!q || !out || !start) return fail(MTTS_E_INVALID, "attention: missing arguments");
   if (((uintptr_t)q & 15) || ldq % 8 || ((uintptr_t)out & 7) || ldo % 4 || ((uintptr_t)mask & 7) || ((uintptr_t)tree & 7))
     return fail(MTTS_E_INVALID, "attention: q 16-byte and out 8-byte aligned, in every row; mask and tree 8-byte");
+  if ((int64_t)B * T > 1 && ldo < (size_t)n_heads * c.D) return fail(MTTS_E_INVALID, "attention: rows of out overlap");
   if (B > 65535) return fail(MTTS_E_UNSUPPORTED, "attention: at most 65,535 rows");
   if ((int64_t)T * n_heads > (1 << 30)) return fail(MTTS_E_INVALID, "attention: too many tokens");
   if (!ws && attn_kv_ws_bytes(B, T, n_heads, c.n_kv, c.D, c.slots, max_len))

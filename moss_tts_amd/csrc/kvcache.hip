@@ -523,7 +523,7 @@ __global__ __launch_bounds__(256) void kv_compact_kernel(KvCompactArgs a) {
   const int D = a.c.D, unit = blockIdx.x >> 1, isv = blockIdx.x & 1, tid = threadIdx.x;
   const int b = unit / a.c.n_kv;
   const int start = a.start[b], n = min(max(a.took[b], 0), a.P), slots = a.c.slots;
-  if (n == 0) return;
+  if (n == 0 || start >= slots) return;  // (nothing of a path behind the cache is a slot)
   const size_t head = (size_t)unit * slots;  // unit = b * n_kv + h
   const bool bf = a.c.type == KV_BF16;
   float* scales = isv ? a.c.vs : a.c.ks;

@@ -11,7 +11,7 @@ attention that reads it.
 Every call runs on the caller's current stream through libmtts.so (include/mtts.h), without a host
 synchronisation, and may be captured into a graph.  `start` (int32 [B], on the device) is the length
 of each row's context: new tokens take the slots behind it.  Rows and slots follow the engine's own
-cache: row b of a batch is row b of the cache.
+cache: row b of a batch is row b of the cache.  Serving only: no gradients are recorded.
 """
 import ctypes
 from typing import List, Optional, Sequence, Tuple
@@ -100,8 +100,8 @@ class Rope:
         self._fn, self._index = N.load().mtts_k_rope, self.device.index
 
     def apply(self, x: torch.Tensor, positions: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """x bf16 [M, H, head_dim] (any strides between tokens and heads) at int32 positions [M];
-        `out` may be x itself."""
+        """x bf16 [M, H, head_dim] (any strides between tokens and heads, 0 too) at int32 positions [M];
+        `out` is x itself or shares no head with it."""
         if x.dim() != 3 or x.dtype is not torch.bfloat16 or x.shape[2] != self.head_dim or x.device != self.device:
             raise ValueError("x is bf16 [tokens, heads, head_dim] on the frequencies' device")
         M, H, D = x.shape

@@ -179,6 +179,24 @@ def test_append_and_move_refusals(N):
                    None)
 
 
+@pytest.mark.parametrize("y,ldy,hsy,M,H", [(FAKE + 64, 128, 64, 2, 2), (FAKE - 126, 128, 64, 2, 2), (FAKE + 4096, 0, 64, 2, 2),
+                                           (FAKE + 4096, 64, 64, 2, 2), (FAKE + 4096, 128, 0, 1, 2),
+                                           (FAKE + 4096, 32, 0, 2, 1), (FAKE + 4096, 96, 64, 3, 2)])
+def test_rope_outputs_that_overlap(N, y, ldy, hsy, M, H):
+    r = N.MttsRope(FAKE, 64, 0, 1.0)
+    with pytest.raises(ValueError, match="overlap"):
+        N.call("mtts_k_rope", FAKE, 128, 64, y, ldy, hsy, FAKE, M, H, 64, ctypes.byref(r), None)
+
+
+def test_output_rows_that_overlap(N):
+    c = ctypes.byref(cache(N))
+    with pytest.raises(ValueError, match="overlap"):
+        N.call("mtts_k_attn_kv", c, FAKE, 256, FAKE, 252, 4, FAKE, None, None, None, 1, 2, 0.0, 0, FAKE, None)
+    with pytest.raises(ValueError, match="overlap"):
+        N.call("mtts_k_kv_append", c, FAKE, 256, FAKE, 128, FAKE, 128, FAKE, 128, 4, None, None, 0.0, None, None, FAKE, None, 2, 1,
+               None)
+
+
 def test_workspace_bytes(N):
     L = N.load()
     assert L.mtts_k_attn_kv_ws_bytes(64, 64, 32, 8, 128, 2048, 0) == 0  # one block a row and KV head: no partials

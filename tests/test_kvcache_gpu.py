@@ -337,7 +337,7 @@ def sees(B, T, slots, start, counts, tree, mask):
             for j in range(min(start[b], slots)):
                 out[b, t, j] = mask is None or bool(mask[b, j])
             for u in range(n):
-                if start[b] + u < slots:
+                if 0 <= start[b] + u < slots:
                     out[b, t, start[b] + u] = (u <= t) if tree is None else bool(tree[b][t] >> u & 1)
     return out
 
@@ -454,6 +454,70 @@ def test_attend_split(kv, kind, B, T, H, Hkv, start, kw):
 def test_attend_large_scores(kv, kind):
     """scores of hundreds: one key takes nearly all, the running maximum moves"""
     attend_case(kv, kind, 1, 9, 4, 1, 128, [500], tree=True, spread=5.0)
+
+
+FAR = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T,G", [(3, 2), (40, 4), (64, 4)])
+@pytest.mark.parametrize("slots", [64, 4096])
+@pytest.mark.parametrize("tree", [False, True])
+def test_starts_outside_the_cache(kv, kind, T, G, slots, tree):
+    """new tokens before slot 0 or behind the last have no slot: nothing is stored for them, read from them or
+    moved to them, and attention sees those tokens that have one"""
+    from tests.kv_layout import contents
+    g = torch.Generator().manual_seed(T + G + slots)
+    start = [-2, 5 - T, -T - 40, slots - 2, slots, FAR, FAR - 7, -FAR - 1]
+    B, D, n_kv = len(start), 64, 2
+    c = fresh(kv, B, n_kv, slots, D, kind)
+    c.write(rnd(g, B, slots, n_kv, D).cuda(), rnd(g, B, slots, n_kv, D).cuda(), i32([0] * B))
+    before = [t.clone() for t in contents(c)]
+    new = rnd(g, B, T, n_kv, D)
+    c.write(new.cuda(), new.cuda(), i32(start))
+    want = stored(new, kind)[0]
+    for x, y in zip(contents(c), before):
+        for b in range(B):
+            for u in range(T):
+                if 0 <= start[b] + u < slots:
+                    y[b, :, start[b] + u] = want[b, u]
+        assert torch.equal(x, y)
+    q = rnd(g, B, T, G * n_kv, D)
+    tr = trees(g, B, T) if tree else None
+    got = c.attend(q.cuda(), i32(start), tree=signed(tr) if tree else None).cpu()
+    o, pv, qk = attend64(q, *before, sees(B, T, slots, start, None, tr, None), D ** -0.5)
+    attention_close(got, o, pv, qk, D)
+    for r in c.read(T, start=i32(start)):
+        for b in range(B):
+            for u in range(T):
+                if not 0 <= start[b] + u < slots:
+                    assert (r[b, :, u] == 0).all()
+    path = torch.arange(T, dtype=torch.int32).repeat(B, 1).flip(1).cuda()
+    c.compact(i32(start), path, i32([T] * B))
+    for x, y in zip(contents(c), before):
+        for b in range(B):
+            old = y[b].clone()
+            for i in range(T):
+                t, f = start[b] + i, start[b] + T - 1 - i
+                if 0 <= t < slots and 0 <= f < slots:
+                    y[b, :, t] = old[:, f]
+        assert torch.equal(x, y)
+
+
+def test_rope_broadcast_and_gaps(kv):
+    """one head's values at every token and head; an output between the input's heads"""
+    g = torch.Generator().manual_seed(1)
+    r, pos = kv.Rope(64, theta=1e4), i32([3, 70, 9])
+    x = rnd(g, 1, 1, 64).cuda()
+    assert torch.equal(r.apply(x.expand(3, 5, 64), pos), r.apply(x.repeat(3, 5, 1), pos))
+    rows = rnd(g, 3, 4, 64).cuda()
+    want = r.apply(rows[:, :2].contiguous(), pos)
+    kept = rows[:, :2].clone()
+    r.apply(rows[:, :2], pos, out=rows[:, 2:])
+    assert torch.equal(rows[:, 2:], want) and torch.equal(rows[:, :2], kept)
+    for bad in (x.expand(3, 5, 64), rows.view(-1)[64 + 32:64 + 32 + 3 * 128].view(3, 2, 64)):
+        with pytest.raises(ValueError, match="overlap"):
+            r.apply(rows.view(-1)[64:64 + 3 * 128].view(3, 2, 64) if bad.shape[1] == 2 else rows[:, :1].expand(3, 5, 64), pos, out=bad)
 
 
 @pytest.mark.parametrize("kind", KINDS)
