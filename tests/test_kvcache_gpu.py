@@ -451,6 +451,40 @@ def test_attend_split(kv, kind, B, T, H, Hkv, start, kw):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("B,T,H,Hkv,start,kw", [
+    (1, 1, 32, 1, [300], dict(masked=True)), (2, 1, 33, 1, [40, 900], {}), (1, 1, 32, 1, [3500], {}),
+    (2, 12, 8, 2, [2100, 40], dict(tree=True, masked=True)), (2, 64, 8, 2, [1500, 2050], dict(tree=True, masked=True, counts=[64, 40])),
+    (1, 64, 16, 2, [1800], dict(tree=True)), (1, 150, 4, 2, [1700], {}), (3, 70, 4, 1, [31, 900, 0], dict(masked=True)),
+    (70, 12, 4, 1, [(97 * b) % 640 for b in range(70)], dict(max_len=2000, counts=[b % 13 for b in range(70)]))])
+def test_attend_groups_and_forms(kv, kind, D, B, T, H, Hkv, start, kw):
+    """groups of a tile of rows and one more; one, two, four and more tiles of rows, split and not"""
+    attend_case(kv, kind, B, T, H, Hkv, D, start, **kw)
+
+
+def test_two_streams_at_once(kv):
+    """calls of two streams over one cache, each with a workspace of its own, as one after the other"""
+    g = torch.Generator().manual_seed(11)
+    c = fresh(kv, 2, 2, 4096, 128, "int8")
+    c.write(rnd(g, 2, 4000, 2, 128).cuda(), rnd(g, 2, 4000, 2, 128).cuda(), i32([0, 0]))
+    qs = [rnd(g, 2, T, 8, 128).cuda() for T in (1, 8, 30, 64)]
+    at = i32([3900, 2500])
+    want = [c.attend(q, at) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(4):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append([c.attend(q, at) for q in (qs if i else qs[::-1])])
+    torch.cuda.synchronize()
+    for run in got[0]:
+        assert all(torch.equal(x, y) for x, y in zip(run[::-1], want))
+    for run in got[1]:
+        assert all(torch.equal(x, y) for x, y in zip(run, want))
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_attend_large_scores(kv, kind):
     """scores of hundreds: one key takes nearly all, the running maximum moves"""
     attend_case(kv, kind, 1, 9, 4, 1, 128, [500], tree=True, spread=5.0)
