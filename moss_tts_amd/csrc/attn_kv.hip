@@ -516,9 +516,46 @@ struct Stage {
   }
 };
 
+// The (m, l, o) of N groups of waves that went through different tiles of the same rows [r0, r1), into one,
+// in order: to the output, or as the partial of a split row (slot >= 0), which the join divides.  src: the
+// first group's o, [rows][D + 4], `step` bytes from one to the next; ml: pairs, `mstep` of them to the next.
+template <int D, int N>
+__device__ __forceinline__ void merge_groups(const AttnKvArgs& a, int b, int hkv, int G, int r0, int r1, int slot, float* po,
+                                             int rows, const char* src, int step, const float* ml, int mstep) {
+  for (int q = threadIdx.x; q < (r1 - r0) * (D / 4); q += blockDim.x) {
+    const int r = q / (D / 4), d = q % (D / 4) * 4;
+    float M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < N; ++w) M = fmaxf(M, ml[(w * mstep + r) * 2]);
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < N; ++w) {
+      const float2 x = *reinterpret_cast<const float2*>(ml + (w * mstep + r) * 2);
+      const float f = x.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x.x - M);
+      const float4 z = *reinterpret_cast<const float4*>(src + (size_t)w * step + (r * (D + 4) + d) * 4);
+      L += f * x.y;
+      y.x += f * z.x; y.y += f * z.y; y.z += f * z.z; y.w += f * z.w;
+    }
+    if (slot >= 0) {
+      *reinterpret_cast<float4*>(po + (size_t)r * D + d) = y;
+      if (d == 0) *reinterpret_cast<float2*>(po + (size_t)rows * D + r * 2) = make_float2(M, L);
+    } else {
+      const float sc = L == 0.f ? 0.f : 1.f / L;  // (a row that saw nothing is 0)
+      const int t = (r0 + r) / G;
+      bf16_t* dst = a.out + ((size_t)b * a.T + t) * a.ldo + (size_t)(hkv * G + r0 + r - t * G) * D + d;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(y.x * sc, y.y * sc), pack2(y.z * sc, y.w * sc));
+    }
+  }
+}
+
 // Up to 32 rows a KV head (a decode step, a small tree): bound by the cache's bytes.  The NW waves of a
 // block take tiles in turn, loaded one tile ahead, with no barrier in the loop, and merge once at the
-// end.  8-bit fragments go from memory straight into registers, bf16 ones through LDS of the wave's own.
+// end.  8-bit fragments go from memory straight into registers, bf16 ones through LDS of the wave's own
+// (straight, a wave-wide load of them touched 64 lines of memory).
+//   Measured with 32 q heads on 8 KV heads of 128, one token a row: 32 rows of 4,000 slots bf16 81 us
+// (4.9 TB/s), e4m3 41 us (5.0 TB/s); one row of 130,000 bf16 114 us (4.7 TB/s, with the join), e4m3 66 us
+// (4.2 TB/s); a large copy reaches 4.9.  One row of 389 bf16 slots 8 us: a chain of dependent loads
+// (length, tiles, merge) and the first fetch of 20 KB of code.
 template <int KT, int D, int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, 2) void attn_kv_keys(AttnKvArgs a, int NS, int least, uint32_t rG) {
   constexpr bool Q8 = KT != KV_BF16;
@@ -668,55 +705,44 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_kv_keys(AttnKvArgs a, int NS,
               make_float4(st.o[t][i], st.o[t][i + 1], st.o[t][i + 2], st.o[t][i + 3]);
     }
     __syncthreads();
-    const bool whole = !SPLIT || sg.slot < 0;
-    float* po = a.part + head_floats(a.B) + (size_t)(sg.slot * Hkv + hkv) * 32 * (D + 2);
-    for (int q = threadIdx.x; q < R * (D / 4); q += 64 * NW) {
-      const int r = q / (D / 4), d = q % (D / 4) * 4;
-      const char* src = lds + (r * (D + 4) + d) * 4;
-      float M = -INFINITY, L = 0.f;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) M = fmaxf(M, mls[w][r][0]);
-      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        const float mw = mls[w][r][0], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - M);
-        const float4 z = *reinterpret_cast<const float4*>(src + w * WL);
-        L += f * mls[w][r][1];
-        y.x += f * z.x; y.y += f * z.y; y.z += f * z.z; y.w += f * z.w;
-      }
-      if (!whole) {  // a split row is divided by the join
-        *reinterpret_cast<float4*>(po + r * D + d) = y;
-        if (d == 0) *reinterpret_cast<float2*>(po + 32 * D + r * 2) = make_float2(M, L);
-      } else {
-        const float sc = L == 0.f ? 0.f : 1.f / L;  // (a row that saw nothing is 0)
-        const int t = r * rG >> 16;
-        bf16_t* dst = a.out + ((size_t)b * a.T + t) * a.ldo + (size_t)(hkv * G + r - t * G) * D + d;
-        *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(y.x * sc, y.y * sc), pack2(y.z * sc, y.w * sc));
-      }
-    }
+    merge_groups<D, NW>(a, b, hkv, G, 0, R, SPLIT ? sg.slot : -1,
+                        a.part + head_floats(a.B) + (size_t)(sg.slot * Hkv + hkv) * 32 * (D + 2), 32, lds, WL, mls[0][0], 32);
     if constexpr (SPLIT) __syncthreads();  // (the next segment writes LDS)
   });
 }
 
-// More rows: bound by the arithmetic on the scores.  The W waves of a block, 32 rows each, go through the
-// same tiles, whose fragments they load, turn into bf16 and put into LDS together, once for all rows, one
-// tile ahead of the products (two LDS buffers, one barrier a tile).
-template <int KT, int D, int W>
-__global__ __launch_bounds__(64 * W, 2) void attn_kv_rows(AttnKvArgs a, int NS, int least, int RB) {
+// More rows: bound by the arithmetic on the scores (of a tile's turn the products take half, the powers, the
+// maximum and the roundings the rest, and two waves a SIMD hide little of one behind the other).  W waves,
+// 32 rows each, go through the same tiles, whose fragments they load, turn into bf16 and put into LDS
+// together, once for all rows, a turn ahead of the products (two halves of LDS, one barrier a turn).
+//   A block has KS such groups, which take the tiles in turn and are merged at the end: with a block each
+// (KS 1), four or two times the partials went through memory: 4 rows of 7,500 e4m3 slots and 16 tokens of
+// 4 heads wrote and read 32 MB of them beside the cache's 50 MB (42 us, 36 like this).
+//   Measured with 32 q heads on 8 KV heads of 128: one row of 130,001 int8 slots, 33 tokens, 160 us
+// (440 TFLOP/s; three of the eight waves have no rows there), 16 rows of 4,000 bf16 slots, 64 tokens, 73 us
+// and 12 for the join (610 TFLOP/s); a large plain matrix product reaches 1,150.
+template <int KT, int D, int W, int KS>
+__global__ __launch_bounds__(64 * W * KS, 2) void attn_kv_rows(AttnKvArgs a, int NS, int least, int RB) {
   constexpr bool Q8 = KT != KV_BF16;
   constexpr int DT = D / 32, rows = 32 * W;
-  constexpr int TT = W == 2 ? 1 : 2;  // tiles a turn (LDS for 4 blocks of 2 waves, or 2 of 4, or 1 of 8)
+  constexpr int TT = W == 2 ? 1 : 2;  // tiles of a group a turn (what LDS holds)
   using St = Stage<KT, D, W>;
-  __shared__ __attribute__((aligned(16))) char lk[2][TT][St::BYTES], lv[2][TT][St::BYTES];
+  constexpr int OS = KS > 1 ? rows * (D + 4) * 4 : 0, GL = 4 * TT * St::BYTES < OS ? OS : 4 * TT * St::BYTES;
+  __shared__ __attribute__((aligned(16))) char lds[KS][GL];  // of a group: two halves of TT tiles, K and V; then its o
+  __shared__ float mls[KS][KS > 1 ? rows : 1][2];
   __shared__ int spared;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wv0 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = wv0 % W, kg = wv0 / W;
+  char* const mylds = lds[kg];
+  auto lk = [&](int half, int i) { return mylds + ((half * TT + i) * 2) * St::BYTES; };
+  auto lv = [&](int half, int i) { return mylds + ((half * TT + i) * 2 + 1) * St::BYTES; };
   const int n = lane & 31, h = lane >> 5;
   const int Hkv = a.c.n_kv, G = a.Hq / Hkv, slots = a.c.slots;
   const Place pl = place_of(NS, least, RB, Hkv);
   if (pl.unit >= NS * Hkv) return;
   const float c = a.scale * 1.44269504088896340736f;
 
-  Segments<6> it(a, NS, least, pl.x, blockIdx.x == 0);
+  Segments<4 + 3 * KS> it(a, NS, least, pl.x, blockIdx.x == 0);
   for (Seg sg; it.next(sg);) {
     const int b = sg.b;
     const RowLen len = sg.len;
@@ -752,25 +778,26 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv_rows(AttnKvArgs a, int NS, 
     auto put = [&](int tile, int half) {
 #pragma unroll
       for (int i = 0; i < TT; ++i) {
-        gk[i].store_k(wave, lane, lk[half][i]);
-        if (gv[i].store_v(a, b, len, min(tile + i, t1 - 1), wv, lane, lv[half][i])) spared = 1;
+        gk[i].store_k(wave, lane, lk(half, i));
+        if (gv[i].store_v(a, b, len, min(tile + i, t1 - 1), wv, lane, lv(half, i))) spared = 1;
         if constexpr (Q8) {
           kn[i] = gk[i].ks * c;
           vn[i] = gk[i].vs;
         }
       }
     };
-    if (t0 < t1) fetch(t0);
+    if (t0 < t1) fetch(t0 + kg * TT);
     bf16x8 qf[D / 16];
     const int tk = myr < Rend ? myr / G : 0;
     const Row row = load_row<D>(a, b, pl.hkv, len, G, tk, myr < Rend ? myr - tk * G : 0, h, qf);
     __syncthreads();  // (spared is 0, and the last segment's tiles have been read)
     loads_done();
     if (t0 < t1) {
-      put(t0, 0);
-      fetch(t0 + TT);
+      put(t0 + kg * TT, 0);
+      fetch(t0 + (KS + kg) * TT);
     }
-    for (int tile = t0, half = 0; tile < t1; tile += TT, half ^= 1) {
+    for (int tb = t0, half = 0; tb < t1; tb += KS * TT, half ^= 1) {
+      const int tile = tb + kg * TT;
       if constexpr (Q8) {
 #pragma unroll
         for (int i = 0; i < TT; ++i) {
@@ -779,16 +806,16 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv_rows(AttnKvArgs a, int NS, 
         }
       }
       __syncthreads();  // this turn's fragments are there, the other half has been read
-      if (tile + TT < t1) {
-        put(tile + TT, half ^ 1);
-        fetch(tile + 2 * TT);
+      if (tb + KS * TT < t1) {
+        put(tile + KS * TT, half ^ 1);
+        fetch(tile + 2 * KS * TT);
       }
       if (act) {
 #pragma unroll
         for (int i = 0; i < TT; ++i) {
           const int tl = tile + i;
           if (tl >= t1) break;
-          const char *kp = lk[half][i] + at, *vp = lv[half][i] + at;
+          const char *kp = lk(half, i) + at, *vp = lv(half, i) + at;
           // (all reads before the first product: one at a time, each product waits out LDS's latency)
           bf16x8 k[D / 16];
 #pragma unroll
@@ -829,13 +856,29 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv_rows(AttnKvArgs a, int NS, 
       __syncthreads();
       if (spared && act)
         for (int tile = max(t0, len.start >> 5); tile < t1; ++tile)
-          add_specials<D>(a, b, len, (const bf16_t*)vb, tile, n, h, row, st.o);
+          if ((tile - t0) / TT % KS == kg) add_specials<D>(a, b, len, (const bf16_t*)vb, tile, n, h, row, st.o);
       if (least) __syncthreads();  // (the next segment clears it)
     }
     st.l = half_sum(st.l);
+    float* po = a.part + head_floats(a.B) + ((size_t)(sg.slot * Hkv + pl.hkv) * RB + pl.rb) * rows * (D + 2);
+    if constexpr (KS > 1) {  // the groups into one
+      __syncthreads();  // (the tiles have been read)
+      if (h == 0) *reinterpret_cast<float2*>(mls[kg][wave * 32 + n]) = make_float2(st.m, st.l);
+      float* os = reinterpret_cast<float*>(mylds) + (wave * 32 + n) * (D + 4) + 4 * h;
+      if (act) {
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<float4*>(os + 32 * t + 2 * i) =
+                make_float4(st.o[t][i], st.o[t][i + 1], st.o[t][i + 2], st.o[t][i + 3]);
+      }
+      __syncthreads();
+      merge_groups<D, KS>(a, b, pl.hkv, G, r0, Rend, sg.slot, po, rows, lds[0], GL, mls[0][0], rows);
+      continue;  // (the next segment writes LDS behind its first barrier)
+    }
     if (myr >= Rend) continue;
     if (sg.slot >= 0) {  // a split row is divided by the join
-      float* po = a.part + head_floats(a.B) + ((size_t)(sg.slot * Hkv + pl.hkv) * RB + pl.rb) * rows * (D + 2);
       const int rr = wave * 32 + n;
       if (h == 0) *reinterpret_cast<float2*>(po + (size_t)rows * D + rr * 2) = make_float2(st.m, st.l);
 #pragma unroll
@@ -857,7 +900,8 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv_rows(AttnKvArgs a, int NS, 
   }
 }
 
-// Joins the partials of a row: GS groups of D / 4 threads (4 dims each) take every GS-th block's partial,
+// Joins the partials of a row.  Bound by their bytes (16 rows x 64 tokens x 32 heads, two blocks a row: 42 MB in
+// 11.6 us) or, for few rows, by the loads' latency: GS groups of D / 4 threads (4 dims each) take every GS-th block's partial,
 // four loads in flight, and the groups' sums are added in order.
 template <int D, int GS>
 __global__ __launch_bounds__(256) void attn_kv_join(AttnKvArgs a, int RB, int rows) {
@@ -937,6 +981,14 @@ __global__ __launch_bounds__(256) void attn_kv_join(AttnKvArgs a, int RB, int ro
 struct AkvPlan {
   int W, RB, NS, least;
 };
+// Constants by measurement, 32 q heads on 8 KV heads of 128, bf16 / e4m3, us:
+//   form: one tile of rows stays with its waves' registers (keys); two as groups of two waves, .. (a group's
+//     rows are a power of two of tiles, so that the tile's loads divide among its waves);
+//   least (tiles a block): 1 row, 16 tokens, 2,000 slots: 8 19.2 / 19.0, 16 21.8 / 21.4; W 8 has no groups
+//     that share a block's tiles: 4;
+//   most (tiles up to which nothing is split): W 2, 1 row of 500 slots: 16 19.6 / 19.4, 32 17.8 / 16.5;
+//     1 row of 2,000: 32 21.8 / 21.4, 64 32.1 / 30.4; W 4, 8 rows of 700: 12 28.6 / 27.1, 24 26.4 / 24.4;
+//     8 rows of 1,400: 24 27.6 / 27.7, 48 37.2 / 35.9.
 static AkvPlan plan(int B, int T, int Hq, int n_kv, int slots, int max_len) {
   AkvPlan p;
   const int64_t R = (int64_t)T * (Hq / n_kv), rt = (R + 31) / 32;
@@ -945,8 +997,8 @@ static AkvPlan plan(int B, int T, int Hq, int n_kv, int slots, int max_len) {
   const int64_t len = std::min<int64_t>(slots, (int64_t)(max_len > 0 ? std::min(max_len, slots) : slots) + T);
   const int64_t tiles = (len + 31) / 32;                              // of the longest row
   const int64_t units = std::max<int64_t>(1, (int64_t)n_kv * p.RB);   // blocks a row, unsplit
-  const int64_t room = 256 * (p.W == 0 ? 1 : 8 / p.W);                // blocks that the card holds at once
-  const int64_t most = p.W == 0 ? 64 : p.W == 8 ? 20 : p.W == 4 ? 12 : 8, least = p.W == 0 || p.W == 2 ? 8 : 4;
+  const int64_t room = 256;                                           // blocks that the card holds at once
+  const int64_t most = p.W == 0 ? 64 : p.W == 8 ? 20 : p.W == 4 ? 24 : 32, least = p.W == 8 ? 4 : 8;
   p.least = (int)least;
   p.NS = (int)std::max<int64_t>(1, std::min(room / units, (int64_t)B * ((tiles + least - 1) / least)));
   // short rows, or enough of them: nothing to join
@@ -972,9 +1024,14 @@ static void launch_form(const AttnKvArgs& a, const AkvPlan& p, int64_t grid, hip
       hipLaunchKernelGGL((attn_kv_keys<KT, D, 8, SPLIT>), dim3(a.c.n_kv, p.NS), dim3(512), 0, s, a, p.NS, p.least, rG);
       break;
     }
-    case 2: hipLaunchKernelGGL((attn_kv_rows<KT, D, 2>), g, dim3(128), 0, s, a, p.NS, p.least, p.RB); break;
-    case 4: hipLaunchKernelGGL((attn_kv_rows<KT, D, 4>), g, dim3(256), 0, s, a, p.NS, p.least, p.RB); break;
-    default: hipLaunchKernelGGL((attn_kv_rows<KT, D, 8>), g, dim3(512), 0, s, a, p.NS, p.least, p.RB);
+    case 2: hipLaunchKernelGGL((attn_kv_rows<KT, D, 2, 4>), g, dim3(512), 0, s, a, p.NS, p.least, p.RB); break;
+    case 4:
+      // (64 rows of 1,000 slots, three row tiles: 52 us in blocks of 4 waves, two a CU, that never wait for
+      // each other, and 67 in blocks of 8; 8 rows of 700, four: 34 and 26)
+      if (!p.least && grid > 256) hipLaunchKernelGGL((attn_kv_rows<KT, D, 4, 1>), g, dim3(256), 0, s, a, p.NS, p.least, p.RB);
+      else hipLaunchKernelGGL((attn_kv_rows<KT, D, 4, 2>), g, dim3(512), 0, s, a, p.NS, p.least, p.RB);
+      break;
+    default: hipLaunchKernelGGL((attn_kv_rows<KT, D, 8, 1>), g, dim3(512), 0, s, a, p.NS, p.least, p.RB);
   }
 }
 template <int KT, int D>

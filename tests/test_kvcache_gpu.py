@@ -462,6 +462,14 @@ def test_attend_groups_and_forms(kv, kind, D, B, T, H, Hkv, start, kw):
     attend_case(kv, kind, B, T, H, Hkv, D, start, **kw)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("B,T,H,Hkv", [(130, 10, 16, 2), (130, 24, 8, 2), (65, 33, 16, 4)])
+def test_attend_many_short_rows(kv, kind, B, T, H, Hkv):
+    """more rows and heads than the card has compute units: three row tiles a block, and others"""
+    attend_case(kv, kind, B, T, H, Hkv, 32, [(7 * b) % 90 for b in range(B)], tree=True,
+                counts=[T - b % 3 if b % 11 else 0 for b in range(B)])
+
+
 def test_two_streams_at_once(kv):
     """calls of two streams over one cache, each with a workspace of its own, as one after the other"""
     g = torch.Generator().manual_seed(11)
