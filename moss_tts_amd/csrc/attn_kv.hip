@@ -300,30 +300,59 @@ struct RowState {
         for (int i = 0; i < 16; ++i) o[t][i] *= al;
     }
   }
-  // probs: vsl this lane's slot's value scale.  p: the operand of the second product.  p is rounded to bf16,
-  // the product's type: half a step of 2^-8 at random signs over the keys, no more than the output's own
-  // rounding; sums stay in 32 bits.
+  // probs: vsl this lane's slot's value scale.  p: the operand of the second product, rounded to bf16, the
+  // product's type: half a step of 2^-8 at random signs over the keys.  l sums the rounded values, so that
+  // a key that takes nearly all keeps nearly all of 1, whatever its rounding (8-bit types: with COMP, which
+  // costs 16 more instructions a tile: 2 % at most where the cache's bytes are the bound, with int8 8 %;
+  // without, the values before rounding).  Sums stay in 32 bits.
+  template <bool COMP>
   __device__ __forceinline__ void probs(const f32x16& s, float c, float vsl, uint32_t sees, bool special, bf16x8* p) {
     constexpr bool Q8 = KT != KV_BF16;
     const float mu = m == -INFINITY ? 0.f : m;
-    float e[16], sum = 0.f;
+    float e[16], sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       e[i] = __builtin_amdgcn_exp2f(Q8 ? s[i] - mu : fmaf(s[i], c, -mu));
-      sum += e[i];
+      if (Q8 && !COMP) sum[0] += e[i];
     }
-    l += sum;
+    float rvs = 0.f;
     if constexpr (Q8) {
+      if (COMP) {
+        vsl = vsl == 0.f ? 1.f : vsl;  // (its codes are 0)
+        rvs = __builtin_amdgcn_rcpf(vsl);
+      }
       unrolled<16>([&](auto i) { e[i.value] *= row_bcast<i.value>(vsl); });
       if (special) {  // some slot's scale is not finite: it counts for the rows that see it alone
 #pragma unroll
         for (int i = 0; i < 16; ++i) e[i] = sees >> i & 1 ? e[i] : 0.f;
       }
     }
+    union {
+      uint32_t w[4];
+      bf16x2 h[4];
+      bf16x8 v;
+    } r[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) p[u][i] = (__bf16)e[8 * u + i];
+      for (int i = 0; i < 8; ++i) r[u].v[i] = (__bf16)e[8 * u + i];
+    p[0] = r[0].v;
+    p[1] = r[1].v;
+    if constexpr (!Q8) {
+      const bf16x2 one = {(__bf16)1.f, (__bf16)1.f};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) sum[u] = __builtin_amdgcn_fdot2_f32_bf16(r[u].h[i], one, sum[u], false);
+    } else if constexpr (COMP) {
+      unrolled<16>([&](auto i) {
+        const uint32_t w = r[i.value >> 3].w[(i.value & 7) >> 1];
+        const float x = __uint_as_float(i.value & 1 ? w & 0xffff0000u : w << 16), y = row_bcast<i.value>(rvs);
+        if (special) sum[i.value & 1] += sees >> i.value & 1 ? x * y : 0.f;
+        else sum[i.value & 1] = fmaf(x, y, sum[i.value & 1]);
+      });
+    }
+    l += sum[0] + sum[1];
   }
 };
 
@@ -671,7 +700,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_kv_keys(AttnKvArgs a, int NS,
       }
       bf16x8 p[2];
       st.scores(s, c, kcl, edge, sees);
-      st.probs(s, c, vsl, sees, special, p);
+      st.template probs<true>(s, c, vsl, sees, special, p);
 #pragma unroll
       for (int t = 0; t < DT; ++t)
 #pragma unroll
@@ -837,7 +866,7 @@ __global__ __launch_bounds__(64 * W * KS, 2) void attn_kv_rows(AttnKvArgs a, int
           }
           st.scores(s, c, ks[i], edge, sees);
           bf16x8 p[2];
-          st.probs(s, c, vsl, sees, special, p);
+          st.template probs<false>(s, c, vsl, sees, special, p);
           bf16x8 v[DT][2];
 #pragma unroll
           for (int t = 0; t < DT; ++t)
