@@ -372,7 +372,8 @@ int mtts_k_kv_compact(const mtts_kv_cache* cache, const int32_t* start_dev, cons
  * context slots j < start[b] with mask[b][j] != 0 (mask uint8 [B][slots], 8-byte aligned, NULL: all) and
  * those new tokens u (slots start[b] + u) with bit u of tree[b][t] (T <= 64), or with tree NULL u <= t
  * (any T).  softmax(scale q . k) v, scale <= 0: 1 / sqrt(head_dim).  A token that sees nothing gets
- * zeros; what it does not see never reaches it, NaN and infinities included.  q / out: token b * T + t
+ * zeros; what it does not see never reaches it, NaN and infinities included (finite values that it sees:
+ * up to 2^100, sums are in 32 bits).  q / out: token b * T + t
  * at + (b * T + t) * ld, [n_heads][head_dim]; rows behind counts[b] are left as they are.
  * max_len: an upper bound of start the caller knows (<= 0: slots); it sizes the launch, not the result.
  * ws_dev: mtts_k_attn_kv_ws_bytes bytes of scratch (0: NULL is fine), not shared by calls that may run
