@@ -24,15 +24,22 @@ DTYPES = {"bf16": 0, "e4m3": 1, "int8": 2}
 TREE_MAX = 64
 
 _KINDS = {"default": 0, "linear": 1, "ntk": 2, "yarn": 3, "llama3": 4}
+_SCALING = {"rope_type", "type", "factor", "original_max_position_embeddings", "beta_fast", "beta_slow", "attention_factor",
+            "low_freq_factor", "high_freq_factor"}
 
 
 def rope_turns(rotary_dim: int, theta: float, scaling: Optional[dict] = None) -> Tuple[torch.Tensor, float]:
     """Host: (revolutions per position of each pair, float64 [rotary_dim / 2]; factor on the rotated
     values).  `scaling` takes the keys of a model config's `rope_scaling` / `rope_parameters`:
     rope_type default, linear, ntk, yarn or llama3; factor; original_max_position_embeddings;
-    beta_fast, beta_slow, attention_factor; low_freq_factor, high_freq_factor."""
+    beta_fast, beta_slow, attention_factor; low_freq_factor, high_freq_factor; rope_theta, if it is
+    theta.  Any other key that is set is refused: it would change the result."""
     sc = None
     if scaling is not None:
+        other = sorted(k for k, v in scaling.items() if v is not None and k not in _SCALING and
+                       not (k == "rope_theta" and float(v) == float(theta)) and not (k == "truncate" and v is True))
+        if other:
+            raise ValueError(f"rope scaling: {other} not supported")
         kind = scaling.get("rope_type", scaling.get("type", "default"))
         if kind not in _KINDS:
             raise ValueError(f"rope_type {kind!r}: one of {sorted(_KINDS)}")

@@ -84,6 +84,17 @@ def test_rope_turns_refusals(kv, rot, theta, sc):
         kv.rope_turns(rot, theta, sc)
 
 
+@pytest.mark.parametrize("extra", [dict(mscale=0.7), dict(truncate=False), dict(partial_rotary_factor=0.5), dict(rope_theta=5e5),
+                                   dict(short_factor=[1.0])])
+def test_rope_scaling_keys(kv, extra):
+    """a key that the frequencies would not follow is refused, not ignored; one that says the same is fine"""
+    sc = dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=4096)
+    with pytest.raises(ValueError, match="not supported"):
+        kv.rope_turns(64, 1e4, {**sc, **extra})
+    a, b = kv.rope_turns(64, 1e4, sc), kv.rope_turns(64, 1e4, {**sc, "rope_theta": 10000, "truncate": True, "mscale": None})
+    assert torch.equal(a[0], b[0]) and a[1] == b[1]
+
+
 def test_tree_masks(kv):
     masks, depth = kv.tree_masks([[-1, 0, 0, 1, 3], [-1, -1, 1, 2, 0]])
     assert masks.tolist() == [[1, 3, 5, 11, 27], [1, 2, 6, 14, 17]]
