@@ -303,8 +303,8 @@ struct RowState {
   // probs: vsl this lane's slot's value scale.  p: the operand of the second product, rounded to bf16, the
   // product's type: half a step of 2^-8 at random signs over the keys.  l sums the rounded values, so that
   // a key that takes nearly all keeps nearly all of 1, whatever its rounding (8-bit types: with COMP, which
-  // costs 16 more instructions a tile: 2 % at most where the cache's bytes are the bound, with int8 8 %;
-  // without, the values before rounding).  Sums stay in 32 bits.
+  // costs 16 more instructions a tile, nothing to 1 us of 42 where the cache's bytes are the bound; without,
+  // the values before rounding).  Sums stay in 32 bits.
   template <bool COMP>
   __device__ __forceinline__ void probs(const f32x16& s, float c, float vsl, uint32_t sees, bool special, bf16x8* p) {
     constexpr bool Q8 = KT != KV_BF16;
@@ -319,7 +319,7 @@ struct RowState {
     if constexpr (Q8) {
       if (COMP) {
         vsl = vsl == 0.f ? 1.f : vsl;  // (its codes are 0)
-        rvs = __builtin_amdgcn_rcpf(vsl);
+        rvs = fabsf(vsl) < INFINITY ? __builtin_amdgcn_rcpf(vsl) : 1.f;  // (1: p says who sees it)
       }
       unrolled<16>([&](auto i) { e[i.value] *= row_bcast<i.value>(vsl); });
       if (special) {  // some slot's scale is not finite: it counts for the rows that see it alone
@@ -348,8 +348,7 @@ struct RowState {
       unrolled<16>([&](auto i) {
         const uint32_t w = r[i.value >> 3].w[(i.value & 7) >> 1];
         const float x = __uint_as_float(i.value & 1 ? w & 0xffff0000u : w << 16), y = row_bcast<i.value>(rvs);
-        if (special) sum[i.value & 1] += sees >> i.value & 1 ? x * y : 0.f;
-        else sum[i.value & 1] = fmaf(x, y, sum[i.value & 1]);
+        sum[i.value & 1] = fmaf(x, y, sum[i.value & 1]);
       });
     }
     l += sum[0] + sum[1];
