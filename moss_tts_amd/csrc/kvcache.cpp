@@ -51,16 +51,22 @@ extern "C" size_t mtts_kv_bytes(int type, int rows, int n_kv, int head_dim, int 
 }
 
 extern "C" int mtts_rope_turns(double theta, int rot, const mtts_rope_scaling* sc, double* turns, float* factor) {
-  if (!turns || !factor || rot < 2 || rot % 2 || !(theta > 1.0)) return fail(MTTS_E_INVALID, "rope: even rotary dim, base > 1");
+  if (!turns || !factor || rot < 2 || rot % 2 || !(theta > 1.0) || !std::isfinite(theta))
+    return fail(MTTS_E_INVALID, "rope: even rotary dim, base > 1");
   const int kind = sc ? sc->kind : MTTS_ROPE_DEFAULT;
   const double two_pi = 6.283185307179586476925286766559;
   if (kind < MTTS_ROPE_DEFAULT || kind > MTTS_ROPE_LLAMA3) return fail(MTTS_E_INVALID, "rope: unknown scaling");
-  if (kind != MTTS_ROPE_DEFAULT && !(sc->factor >= 1.0)) return fail(MTTS_E_INVALID, "rope: scaling factor >= 1");
-  if ((kind == MTTS_ROPE_YARN || kind == MTTS_ROPE_LLAMA3) && !(sc->original_max_position > 0))
+  if (kind != MTTS_ROPE_DEFAULT && !(sc->factor >= 1.0 && std::isfinite(sc->factor)))
+    return fail(MTTS_E_INVALID, "rope: a finite scaling factor >= 1");
+  if ((kind == MTTS_ROPE_YARN || kind == MTTS_ROPE_LLAMA3) &&
+      !(sc->original_max_position > 0 && std::isfinite(sc->original_max_position)))
     return fail(MTTS_E_INVALID, "rope: the original length is required");
-  if (kind == MTTS_ROPE_YARN && !(sc->beta_fast > 0 && sc->beta_slow > 0))
-    return fail(MTTS_E_INVALID, "rope: beta_fast and beta_slow > 0");
-  if (kind == MTTS_ROPE_LLAMA3 && !(sc->high_freq > sc->low_freq)) return fail(MTTS_E_INVALID, "rope: high_freq > low_freq");
+  if (kind == MTTS_ROPE_YARN && !(sc->beta_slow > 0 && sc->beta_fast >= sc->beta_slow && std::isfinite(sc->beta_fast)))
+    return fail(MTTS_E_INVALID, "rope: beta_fast >= beta_slow > 0");
+  if (kind == MTTS_ROPE_YARN && !std::isfinite(sc->attention_factor))
+    return fail(MTTS_E_INVALID, "rope: a finite attention factor");
+  if (kind == MTTS_ROPE_LLAMA3 && !(sc->high_freq > sc->low_freq && std::isfinite(sc->low_freq) && std::isfinite(sc->high_freq)))
+    return fail(MTTS_E_INVALID, "rope: high_freq > low_freq");
   if (kind == MTTS_ROPE_NTK && rot == 2) return fail(MTTS_E_INVALID, "rope: ntk scaling needs more than one pair");
   *factor = 1.f;
   const double base = kind == MTTS_ROPE_NTK ? theta * std::pow(sc->factor, rot / (rot - 2.0)) : theta;

@@ -24,30 +24,43 @@ DTYPES = {"bf16": 0, "e4m3": 1, "int8": 2}
 TREE_MAX = 64
 
 _KINDS = {"default": 0, "linear": 1, "ntk": 2, "yarn": 3, "llama3": 4}
-_SCALING = {"rope_type", "type", "factor", "original_max_position_embeddings", "beta_fast", "beta_slow", "attention_factor",
-            "low_freq_factor", "high_freq_factor"}
+# (attention_factor 0: by the formula)
+_DEFAULTS = {"factor": 1.0, "original_max_position_embeddings": 0.0, "beta_fast": 32.0, "beta_slow": 1.0,
+             "attention_factor": 0.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0}
+_SCALING = {"rope_type", "type", *_DEFAULTS}
 
 
 def rope_turns(rotary_dim: int, theta: float, scaling: Optional[dict] = None) -> Tuple[torch.Tensor, float]:
     """Host: (revolutions per position of each pair, float64 [rotary_dim / 2]; factor on the rotated
     values).  `scaling` takes the keys of a model config's `rope_scaling` / `rope_parameters`:
-    rope_type default, linear, ntk, yarn or llama3; factor; original_max_position_embeddings;
-    beta_fast, beta_slow, attention_factor; low_freq_factor, high_freq_factor; rope_theta, if it is
-    theta.  Any other key that is set is refused: it would change the result."""
+    rope_type (or type) default, linear, ntk, yarn or llama3; factor, and for yarn and llama3
+    original_max_position_embeddings, which are required; beta_fast (32), beta_slow (1),
+    attention_factor (0.1 ln(factor) + 1); low_freq_factor (1), high_freq_factor (4); rope_theta, if it
+    is theta.  None is as a key that is not there; any other key that is set is refused: it would
+    change the result."""
     sc = None
     if scaling is not None:
-        other = sorted(k for k, v in scaling.items() if v is not None and k not in _SCALING and
+        scaling = {k: v for k, v in scaling.items() if v is not None}
+        other = sorted(k for k, v in scaling.items() if k not in _SCALING and
                        not (k == "rope_theta" and float(v) == float(theta)) and not (k == "truncate" and v is True))
         if other:
             raise ValueError(f"rope scaling: {other} not supported")
-        kind = scaling.get("rope_type", scaling.get("type", "default"))
+        kinds = {scaling[k] for k in ("rope_type", "type") if k in scaling}
+        _need(len(kinds) < 2, f"rope scaling: two types, {sorted(map(str, kinds))}")
+        kind = kinds.pop() if kinds else "default"
         if kind not in _KINDS:
             raise ValueError(f"rope_type {kind!r}: one of {sorted(_KINDS)}")
-        sc = N.MttsRopeScaling(_KINDS[kind], float(scaling.get("factor", 1.0)),
-                               float(scaling.get("original_max_position_embeddings", 0) or 0),
-                               float(scaling.get("beta_fast") or 32.0), float(scaling.get("beta_slow") or 1.0),
-                               float(scaling.get("low_freq_factor", 1.0)), float(scaling.get("high_freq_factor", 4.0)),
-                               float(scaling.get("attention_factor") or 0.0))
+        if kind == "default":  # (a scaling that lost its type, or a factor that would not be applied)
+            lost = not ("rope_type" in scaling or "type" in scaling)
+            given = sorted(k for k in scaling if k in _DEFAULTS and
+                           (lost or k in ("factor", "attention_factor") and scaling[k] != 1))
+            _need(not given, f"rope scaling: {given} without a type that uses them")
+        else:
+            _need("factor" in scaling, f"rope scaling: {kind} needs its factor")
+        at = {k: float(scaling.get(k, d)) for k, d in _DEFAULTS.items()}
+        _need("attention_factor" not in scaling or at["attention_factor"] > 0, "rope scaling: attention_factor > 0")
+        sc = N.MttsRopeScaling(_KINDS[kind], at["factor"], at["original_max_position_embeddings"], at["beta_fast"],
+                               at["beta_slow"], at["low_freq_factor"], at["high_freq_factor"], at["attention_factor"])
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError("rotary_dim is even and at least 2")
     turns = torch.empty(rotary_dim // 2, dtype=torch.float64)

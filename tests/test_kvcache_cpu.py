@@ -95,6 +95,60 @@ def test_rope_scaling_keys(kv, extra):
     assert torch.equal(a[0], b[0]) and a[1] == b[1]
 
 
+NAN, INF = float("nan"), float("inf")
+YARN = dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=4096)
+LLAMA3 = dict(rope_type="llama3", factor=8.0, original_max_position_embeddings=8192)
+
+
+@pytest.mark.parametrize("sc", [
+    dict(rope_type="linear"), dict(rope_type="ntk"), dict(rope_type="ntk", factor=None), {**YARN, "factor": None},
+    dict(rope_type="yarn", original_max_position_embeddings=4096), dict(rope_type="llama3", original_max_position_embeddings=8192),
+    dict(factor=4.0), dict(rope_type="default", factor=4.0), dict(rope_type="default", attention_factor=1.2), dict(original_max_position_embeddings=4096),
+    dict(type="ntk", rope_type="linear", factor=2.0), {**YARN, "beta_fast": 0}, {**YARN, "beta_slow": 0},
+    {**YARN, "beta_slow": -1.0}, {**YARN, "beta_fast": 1, "beta_slow": 32}, {**YARN, "attention_factor": 0},
+    {**YARN, "attention_factor": -1.0}, {**YARN, "attention_factor": NAN}, {**YARN, "attention_factor": INF},
+    {**YARN, "factor": INF}, {**YARN, "factor": NAN}, {**YARN, "beta_fast": NAN}, {**YARN, "beta_fast": INF},
+    {**YARN, "original_max_position_embeddings": INF}, {**YARN, "original_max_position_embeddings": None},
+    {**YARN, "original_max_position_embeddings": 0}, dict(rope_type="linear", factor=INF), {**LLAMA3, "high_freq_factor": INF},
+    {**LLAMA3, "low_freq_factor": NAN}, {**LLAMA3, "low_freq_factor": 5.0}])
+def test_rope_scaling_is_never_made_up(kv, sc):
+    """what a scaling needs has to be there, and a value that is there is used or refused"""
+    with pytest.raises(ValueError):
+        kv.rope_turns(64, 1e4, sc)
+
+
+@pytest.mark.parametrize("theta", [INF, 1.0, 0.5, NAN])
+def test_rope_base_refused(kv, theta):
+    with pytest.raises(ValueError):
+        kv.rope_turns(64, theta)
+
+
+@pytest.mark.parametrize("sc", [dict(rope_type="linear", factor=2.0), dict(rope_type="ntk", factor=2.0), YARN, LLAMA3,
+                                dict(rope_type="default"), {}])
+def test_rope_scaling_none_is_absent(kv, sc):
+    """a key that holds None is as one that is not there, every key alike"""
+    keys = ("type", "beta_fast", "beta_slow", "attention_factor", "low_freq_factor", "high_freq_factor", "factor",
+            "original_max_position_embeddings", "rope_theta", "rope_type")
+    a, b = kv.rope_turns(64, 1e4, sc), kv.rope_turns(64, 1e4, {**{k: None for k in keys}, **sc})
+    assert torch.equal(a[0], b[0]) and a[1] == b[1]
+    if "rope_type" in sc:  # the older name of the key; both, if they agree
+        old = {"type" if k == "rope_type" else k: v for k, v in sc.items()}
+        for other in (old, {**old, "rope_type": None}, {**old, "rope_type": sc["rope_type"]}):
+            c = kv.rope_turns(64, 1e4, other)
+            assert torch.equal(a[0], c[0]) and a[1] == c[1]
+
+
+def test_rope_explicit_values_are_used(kv):
+    plain = kv.rope_turns(64, 1e4)[0]
+    assert torch.equal(kv.rope_turns(64, 1e4, dict(rope_type="default", factor=1.0, original_max_position_embeddings=4096))[0], plain)
+    for sc in ({**LLAMA3, "low_freq_factor": 0}, {**LLAMA3, "low_freq_factor": 2.0, "high_freq_factor": 3.0},
+               {**YARN, "beta_fast": 8, "beta_slow": 0.5, "attention_factor": 1e-3}):
+        turns, factor = kv.rope_turns(64, 1e4, sc)
+        want, m = formula(64, 1e4, sc)
+        assert torch.allclose(turns * 2 * math.pi, torch.tensor(want, dtype=torch.float64), rtol=1e-13, atol=0)
+        assert abs(factor - m) <= 2.0 ** -24 * m
+
+
 def test_tree_masks(kv):
     masks, depth = kv.tree_masks([[-1, 0, 0, 1, 3], [-1, -1, 1, 2, 0]])
     assert masks.tolist() == [[1, 3, 5, 11, 27], [1, 2, 6, 14, 17]]
