@@ -1,4 +1,5 @@
 // C ABI of the drafted-token operators (include/mtts.h): argument checks and launches.
+#include <algorithm>
 #include <cmath>
 
 #include "engine_internal.h"
@@ -36,6 +37,64 @@ bool rope_of(const mtts_rope* r, int D, RopeView* v) {
 bool apart(int n, size_t ld, int m, size_t hs, size_t d) {
   if (n > 1 && m > 1) return (hs >= d && ld >= (m - 1) * hs + d) || (ld >= d && hs >= (n - 1) * ld + d);
   return (n < 2 || ld >= d) && (m < 2 || hs >= d);
+}
+
+
+// The bytes of a tensor argument: n[0] x n[1] runs of `run` bytes, s[i] bytes apart.
+struct Runs {
+  uintptr_t at;
+  int64_t run, s[2], n[2];
+  Runs(const void* p, int n0, size_t s0, int n1, size_t s1, int64_t d)  // in elements of 2 bytes
+      : at((uintptr_t)p), run(2 * d), s{2 * (int64_t)s0, 2 * (int64_t)s1}, n{n0, n1} {
+    // runs that touch or lie in one another are one
+    for (int again = 0; again < 2; ++again)
+      for (int i = 0; i < 2; ++i)
+        if (s[i] <= run || n[i] < 2) {
+          run += (n[i] - 1) * (n[i] < 2 ? 0 : s[i]);
+          n[i] = 1;
+          s[i] = 0;
+        }
+  }
+  int64_t end() const { return (n[0] - 1) * s[0] + (n[1] - 1) * s[1] + run; }
+};
+// whether lo < c + sum of s t < hi for some t, from t.lo to t.hi each; strides in falling order
+struct Term {
+  int64_t s, lo, hi;
+};
+bool hits(const Term* t, int n, int64_t c, int64_t lo, int64_t hi) {
+  if (n == 0) return lo < c && c < hi;
+  int64_t least = c, most = c;
+  for (int i = 1; i < n; ++i) {
+    least += t[i].s * t[i].lo;
+    most += t[i].s * t[i].hi;
+  }
+  const auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };
+  const int64_t first = std::max(t->lo, -floor_div(most - lo - 1, t->s)), last = std::min(t->hi, floor_div(hi - 1 - least, t->s));
+  for (int64_t x = first; x <= last; ++x)
+    if (hits(t + 1, n - 1, c + x * t->s, lo, hi)) return true;
+  return false;
+}
+// whether two arguments share a byte: at once if their extents do not meet (nearly every call), else by the
+// differences of their runs' places
+bool share(const Runs& a, const Runs& b) {
+  const int64_t c = (int64_t)(b.at - a.at);
+  if (c >= a.end() || -c >= b.end()) return false;
+  Term t[4];
+  int n = 0;
+  const auto add = [&](int64_t s, int64_t lo, int64_t hi) {
+    if (lo == hi) return;
+    for (int i = 0; i < n; ++i)
+      if (t[i].s == s) {
+        t[i].lo += lo;
+        t[i].hi += hi;
+        return;
+      }
+    t[n++] = Term{s, lo, hi};
+  };
+  for (int i = 0; i < 2; ++i) add(a.s[i], 1 - a.n[i], 0);
+  for (int i = 0; i < 2; ++i) add(b.s[i], 0, b.n[i] - 1);
+  std::sort(t, t + n, [](const Term& x, const Term& y) { return x.s > y.s; });
+  return hits(t, n, c, -b.run, a.run);
 }
 
 }  // namespace
@@ -101,12 +160,14 @@ extern "C" int mtts_k_rope(const uint16_t* x, size_t ldx, size_t hsx, uint16_t* 
   if (M < 0 || H < 0 || D < 2 || D % 2) return fail(MTTS_E_INVALID, "rope: bad sizes");
   if (M == 0 || H == 0) return 0;
   RopeArgs a{x, y, ldx, hsx, ldy, hsy, pos, M, H, D, {}};
-  if (!x || !y || !pos || !rope || !rope_of(rope, D, &a.r)) return fail(MTTS_E_INVALID, "rope: bad arguments");
-  if (x == y && (ldx != ldy || hsx != hsy)) return fail(MTTS_E_INVALID, "rope: in place needs the same strides");
+  if (!x || !y || !pos || !rope) return fail(MTTS_E_INVALID, "rope: bad arguments");
   if (!apart(M, ldy, H, hsy, D)) return fail(MTTS_E_INVALID, "rope: the output's heads overlap");
-  // an output inside the input's extent, but not between its heads, would be read after it was written
-  const uintptr_t x0 = (uintptr_t)x, y0 = (uintptr_t)y, gap = x0 < y0 ? y0 - x0 : x0 - y0;
-  if (x != y && gap < 2 * (size_t)D) return fail(MTTS_E_INVALID, "rope: the output overlaps the input");
+  // (a wave rotates a head in its registers: in place it is read before it is written; any other head that is
+  // shared would be read by one wave before or after another has written it)
+  const bool in_place = x == y && (M == 1 || ldx == ldy) && (H == 1 || hsx == hsy);
+  if (!in_place && share(Runs(x, M, ldx, H, hsx, D), Runs(y, M, ldy, H, hsy, D)))
+    return fail(MTTS_E_INVALID, "rope: the output overlaps the input (in place is fine, with its strides)");
+  if (!rope_of(rope, D, &a.r)) return fail(MTTS_E_INVALID, "rope: bad arguments");
   HIPCHK(rope_apply(a, (hipStream_t)stream));
   return 0;
 }

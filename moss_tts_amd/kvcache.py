@@ -121,7 +121,7 @@ class Rope:
 
     def apply(self, x: torch.Tensor, positions: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """x bf16 [M, H, head_dim] (any strides between tokens and heads, 0 too) at int32 positions [M];
-        `out` is x itself or shares no head with it."""
+        `out` is x itself or shares no head with it (others are refused)."""
         if x.dim() != 3 or x.dtype is not torch.bfloat16 or x.shape[2] != self.head_dim or x.device != self.device:
             raise ValueError("x is bf16 [tokens, heads, head_dim] on the frequencies' device")
         M, H, D = x.shape

@@ -3,6 +3,7 @@ refusals of the C entry points (every check comes before any device call)."""
 import ctypes
 import math
 import os
+import random
 
 import pytest
 
@@ -251,6 +252,60 @@ def test_rope_outputs_that_overlap(N, y, ldy, hsy, M, H):
     r = N.MttsRope(FAKE, 64, 0, 1.0)
     with pytest.raises(ValueError, match="overlap"):
         N.call("mtts_k_rope", FAKE, 128, 64, y, ldy, hsy, FAKE, M, H, 64, ctypes.byref(r), None)
+
+
+def heads_of(base, ld, hs, M, H, D):
+    """every element that a layout touches"""
+    return {base + m * ld + h * hs + d for m in range(M) for h in range(H) for d in range(D)}
+
+
+def rope_accepts(N, x, ldx, hsx, y, ldy, hsy, M, H, D):
+    """whether the overlap checks let a call through (elements from FAKE on); a rotary dim that is refused
+    behind them keeps it from a launch"""
+    with pytest.raises(ValueError) as e:
+        N.call("mtts_k_rope", FAKE + 2 * x, ldx, hsx, FAKE + 2 * y, ldy, hsy, FAKE, M, H, D, ctypes.byref(N.MttsRope(FAKE, 3, 0, 1.0)),
+               None)
+    assert "overlap" in str(e.value) or "arguments" in str(e.value)
+    return "overlap" not in str(e.value)
+
+
+@pytest.mark.parametrize("x,ldx,hsx,y,ldy,hsy,M,H,ok", [
+    (0, 256, 64, 64, 256, 64, 2, 2, False),       # by a whole head
+    (0, 128, 64, 128, 128, 64, 4, 2, False),      # by a whole token
+    (128, 128, 64, 0, 128, 64, 4, 2, False),      # the other way
+    (0, 128, 64, 3 * 128, 128, 64, 4, 2, False),  # the last token alone
+    (0, 128, 64, 4 * 128, 128, 64, 4, 2, True),   # behind it
+    (0, 256, 64, 128, 256, 64, 3, 2, True),       # between the heads of packed rows
+    (0, 256, 0, 128, 256, 64, 3, 2, True),        # one head at every place
+    (0, 0, 0, 128, 256, 64, 3, 2, True), (130, 0, 0, 0, 128, 64, 3, 2, False),
+    (0, 128, 64, 0, 128, 64, 4, 2, True),         # in place
+    (0, 128, 64, 0, 64, 128, 2, 2, False),        # the same elements in another order
+    (0, 999, 64, 0, 7, 64, 1, 2, True),           # in place: the stride of a single token is no stride
+    (0, 128, 64, 0, 128, 999, 2, 1, True), (0, 128, 64, 0, 192, 64, 2, 2, False)])
+def test_rope_output_shares_no_head(N, x, ldx, hsx, y, ldy, hsy, M, H, ok):
+    assert rope_accepts(N, x, ldx, hsx, y, ldy, hsy, M, H, 64) == ok
+
+
+def test_rope_overlap_is_exact(N):
+    """random layouts against every element that they touch"""
+    r = random.Random(5)
+    seen = [0, 0]
+    for _ in range(3000):
+        D, M, H = r.choice([2, 4, 6]), r.randint(1, 5), r.randint(1, 5)
+        ldx, hsx = (r.choice([0, D, H * D, M * D, r.randint(0, 40), 2 * H * D]) for _ in range(2))
+        ldy, hsy = r.choice([(H * D, D), (D, M * D), (2 * H * D, D), (2 * H * D + 3, 2 * D), (ldx, hsx), (D + 1, M * (D + 1))])
+        x, y = r.randint(0, 60), r.randint(0, 60)
+        tok, head = (M, ldy), (H, hsy)
+        if not any(
+                (na == 1 or sa >= D) and (nb == 1 or sb >= (na - 1) * (sa if na > 1 else 0) + D)
+                for (na, sa), (nb, sb) in ((tok, head), (head, tok))):
+            continue  # (the output's own heads overlap, or its tokens interlock)
+        ey = heads_of(y, ldy, hsy, M, H, D)
+        same = x == y and (ldx == ldy or M == 1) and (hsx == hsy or H == 1)
+        ok = same or not ey & heads_of(x, ldx, hsx, M, H, D)
+        assert rope_accepts(N, x, ldx, hsx, y, ldy, hsy, M, H, D) == ok, (x, ldx, hsx, y, ldy, hsy, M, H, D)
+        seen[ok] += 1
+    assert min(seen) > 300, seen
 
 
 def test_output_rows_that_overlap(N):

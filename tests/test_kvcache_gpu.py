@@ -562,6 +562,26 @@ def test_rope_broadcast_and_gaps(kv):
             r.apply(rows.view(-1)[64:64 + 3 * 128].view(3, 2, 64) if bad.shape[1] == 2 else rows[:, :1].expand(3, 5, 64), pos, out=bad)
 
 
+def test_rope_outputs_that_share_heads(kv):
+    """an output shifted by a head or a token is refused, and nothing is written; one between the input's heads
+    or behind its tokens is as a new one"""
+    g = torch.Generator().manual_seed(3)
+    r, pos = kv.Rope(64, theta=1e4), i32([3, 70, 9])
+    buf = rnd(g, 6, 4, 64).cuda()
+    keep = buf.clone()
+    for x, out in ((buf[:3, :2], buf[:3, 1:3]), (buf[:3], buf[1:4]), (buf[1:4], buf[:3]), (buf[:3], buf[2:5]),
+                   (buf[:3, 1:3], buf[:3, :2]), (buf[1:2].expand(3, 4, 64), buf[:3])):
+        with pytest.raises(ValueError, match="overlap"):
+            r.apply(x, pos, out=out)
+        assert torch.equal(buf, keep)
+    for x, out in ((buf[:3], buf[3:]), (buf[:3, :1].expand(3, 2, 64), buf[:3, 2:]), (buf[5:, 1:2].expand(3, 3, 64), buf[:3, :3]),
+                   (buf[:3, ::2], buf[:3, 1::2])):
+        buf.copy_(keep)
+        want = r.apply(x.contiguous(), pos)
+        r.apply(x, pos, out=out)
+        assert torch.equal(out, want)
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_nothing_seen_is_zero(kv, kind):
     c = fresh(kv, 2, 1, 256, 64, kind)
