@@ -352,7 +352,8 @@ int mtts_k_rope(const uint16_t* x, size_t ldx, size_t hsx, uint16_t* y, size_t l
  * start[b] + t.  q, k, v: token b * S + t at + (b * S + t) * ld, heads head_dim apart (the three may lie
  * in one packed row).  k: RMSNorm over the head with weight kn_w (NULL: none), rotation (rope NULL:
  * none) at pos_dev [B * S] (NULL: the slot), then quantised; v: quantised.  q (NULL: none): the same
- * norm (qn_w) and rotation, to q_out in bf16; rows behind counts[b] are left as they are.
+ * norm (qn_w) and rotation, to q_out in bf16; rows behind counts[b] are left as they are.  q_out is q with
+ * its stride, or shares nothing with q, k and v.
  * A head's values are stored as code * scale, scale = max|x| / Q, code = nearest(x Q / max|x|), Q = 448
  * (e4m3) or 127 (int8); a head below 2^-100 as zeros, one with a NaN or an infinity as NaN in whole. */
 int mtts_k_kv_append(const mtts_kv_cache* cache, const uint16_t* q, size_t ldq, const uint16_t* k, size_t ldk,

@@ -182,6 +182,14 @@ extern "C" int mtts_k_kv_append(const mtts_kv_cache* cache, const uint16_t* q, s
   if (B == 0 || S == 0) return 0;
   if (!k || !v || !start || (q && (!q_out || n_heads < 1))) return fail(MTTS_E_INVALID, "append: missing arguments");
   if (q && (int64_t)B * S > 1 && ldqo < (size_t)n_heads * c.D) return fail(MTTS_E_INVALID, "append: rows of q_out overlap");
+  // (q may be rotated in place; the heads of other waves and the keys' and values' blocks may not be written)
+  if (q && B * (int64_t)S <= INT_MAX) {
+    const int M = B * S;
+    const Runs o(q_out, M, ldqo, 1, 0, (int64_t)n_heads * c.D);
+    if ((!(q == q_out && (M == 1 || ldq == ldqo)) && share(Runs(q, M, ldq, 1, 0, (int64_t)n_heads * c.D), o)) ||
+        share(Runs(k, M, ldk, 1, 0, (int64_t)c.n_kv * c.D), o) || share(Runs(v, M, ldv, 1, 0, (int64_t)c.n_kv * c.D), o))
+      return fail(MTTS_E_INVALID, "append: q_out overlaps q, k or v (q in place is fine, with its stride)");
+  }
   KvAppendArgs a{c, q, k, v, ldq, ldk, ldv, q_out, ldqo, n_heads, qn, kn, eps, {}, pos, start, counts, B, S};
   if (!rope_of(rope, c.D, &a.r)) return fail(MTTS_E_INVALID, "append: rotary dim is even and at most the head's");
   HIPCHK(kv_append(a, (hipStream_t)stream));

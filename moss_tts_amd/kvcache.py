@@ -232,7 +232,7 @@ class KVCache:
         """qkv bf16 [B, S, (n_heads + 2 n_kv) * head_dim], the output of the q|k|v projection: norms and
         rotates q and k (positions int32 [B, S]; None: the slots), stores k and v at slots start[b] ..,
         returns q [B, S, n_heads, head_dim].  Rows behind counts[b] (int32 [B]; None: S) store nothing;
-        their q is zero, or what `out` held."""
+        their q is zero, or what `out` held (`out` shares nothing with qkv)."""
         D = self.head_dim
         if (qkv.dim() != 3 or qkv.dtype is not torch.bfloat16 or qkv.device != self.device or n_heads < 1 or
                 qkv.shape[2] != (n_heads + 2 * self.n_kv) * D):

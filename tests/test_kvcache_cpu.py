@@ -308,6 +308,30 @@ def test_rope_overlap_is_exact(N):
     assert min(seen) > 300, seen
 
 
+def append_accepts(N, q, k, v, out, ldq, ldkv, ldo, B, S, H):
+    """as rope_accepts; 2 KV heads of 64"""
+    with pytest.raises(ValueError) as e:
+        N.call("mtts_k_kv_append", ctypes.byref(cache(N)), FAKE + 2 * q, ldq, FAKE + 2 * k, ldkv, FAKE + 2 * v, ldkv, FAKE + 2 * out,
+               ldo, H, None, None, 0.0, ctypes.byref(N.MttsRope(FAKE, 3, 0, 1.0)), None, FAKE, None, B, S, None)
+    assert "overlap" in str(e.value) or "rotary" in str(e.value)
+    return "overlap" not in str(e.value)
+
+
+@pytest.mark.parametrize("q,k,v,out,ldq,ldkv,ldo,B,S,ok", [
+    (0, 256, 384, 0, 512, 512, 512, 2, 3, True),      # packed rows, q in place
+    (0, 256, 384, 4096, 512, 512, 256, 2, 3, True),
+    (0, 256, 384, 512, 512, 512, 512, 1, 2, False),   # the next token's q
+    (0, 256, 384, 64, 512, 512, 512, 1, 1, False),    # by a head
+    (0, 256, 384, 256, 512, 512, 512, 1, 1, False),   # k
+    (0, 256, 384, 384, 512, 512, 512, 1, 1, False),   # v, and what is behind it
+    (0, 256, 384, 512, 512, 512, 256, 1, 1, True), (0, 256, 384, 0, 512, 512, 256, 1, 2, False),
+    (0, 256, 384, 0, 512, 512, 256, 1, 1, True),      # one token: no stride
+    (0, 256, 384, 512, 768, 768, 768, 1, 3, True),    # between the rows' q|k|v
+    (0, 256, 384, 513, 768, 768, 768, 1, 3, False), (0, 256, 384, 513, 768, 768, 768, 1, 1, True)])
+def test_append_output_is_apart(N, q, k, v, out, ldq, ldkv, ldo, B, S, ok):
+    assert append_accepts(N, q, k, v, out, ldq, ldkv, ldo, B, S, 4) == ok
+
+
 def test_output_rows_that_overlap(N):
     c = ctypes.byref(cache(N))
     with pytest.raises(ValueError, match="overlap"):

@@ -302,6 +302,30 @@ def test_append_strided_rows(kv):
         assert all(torch.equal(a, b) for a, b in zip(now, want))
 
 
+@pytest.mark.parametrize("B,S", [(1, 1), (2, 5)])
+def test_append_outputs_that_share(kv, B, S):
+    """q rotated where it lies is as into a new tensor; an output elsewhere inside qkv is refused"""
+    import ctypes
+    from moss_tts_amd import _native as N
+    g = torch.Generator().manual_seed(9)
+    H, Hkv, D = 4, 2, 64
+    W = (H + 2 * Hkv) * D
+    qkv, qn = rnd(g, B, S, W).cuda(), rnd(g, D).cuda()
+    r, at = kv.Rope(D, rotary_dim=32), i32([3] * B)
+    one, two = (fresh(kv, B, Hkv, 64, D, "int8") for _ in range(2))
+    want = one.append(qkv, at, H, rope=r, q_norm=qn)
+    for off in (D, W - H * D):
+        flat = qkv.view(-1)[off:]
+        if flat.numel() >= B * S * H * D:
+            with pytest.raises(ValueError, match="overlap"):
+                two.append(qkv, at, H, rope=r, q_norm=qn, out=flat[:B * S * H * D].view(B, S, H, D))
+    p = qkv.data_ptr()
+    N.call("mtts_k_kv_append", two._ref, p, W, p + 2 * H * D, W, p + 2 * (H + Hkv) * D, W, p, W, H, qn.data_ptr(), None, 1e-6,
+           ctypes.byref(r._c), None, at.data_ptr(), None, B, S, torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(qkv.view(B, S, -1, D)[:, :, :H], want)
+    assert all(torch.equal(x, y) for x, y in zip(raw(one), raw(two)))
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("P,path,took,start", [(1, [[0]], [1], [3]), (5, [[0, 2, 4, 1, 1], [1, 0, 3, 3, 2]], [3, 5], [30, 0]),
                                                (64, None, [64, 20], [1, 190]), (4, [[0, 63, -1, 64], [2, 1, 0, 3]], [4, -2], [60, 5]),
