@@ -375,7 +375,8 @@ int mtts_k_kv_compact(const mtts_kv_cache* cache, const int32_t* start_dev, cons
  * (any T).  softmax(scale q . k) v, scale <= 0: 1 / sqrt(head_dim).  A token that sees nothing gets
  * zeros; what it does not see never reaches it, NaN and infinities included (finite values that it sees:
  * up to 2^100, sums are in 32 bits).  q / out: token b * T + t
- * at + (b * T + t) * ld, [n_heads][head_dim]; rows behind counts[b] are left as they are.
+ * at + (b * T + t) * ld, [n_heads][head_dim]; rows behind counts[b] are left as they are; out is q with its
+ * stride, or shares nothing with it.
  * max_len: an upper bound of start the caller knows (<= 0: slots); it sizes the launch, not the result.
  * ws_dev: mtts_k_attn_kv_ws_bytes bytes of scratch (0: NULL is fine), not shared by calls that may run
  * at once; nothing is kept in it.  At most 65,535 rows. */

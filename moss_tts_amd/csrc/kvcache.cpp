@@ -237,6 +237,10 @@ extern "C" int mtts_k_attn_kv(const mtts_kv_cache* cache, const uint16_t* q, siz
   if ((int64_t)B * T > 1 && ldo < (size_t)n_heads * c.D) return fail(MTTS_E_INVALID, "attention: rows of out overlap");
   if (B > 65535) return fail(MTTS_E_UNSUPPORTED, "attention: at most 65,535 rows");
   if ((int64_t)T * n_heads > (1 << 30)) return fail(MTTS_E_INVALID, "attention: too many tokens");
+  // (a block reads the q of the rows that it writes, before it writes them: in place is fine)
+  if (B * (int64_t)T <= INT_MAX && !(q == out && ((int64_t)B * T == 1 || ldq == ldo)) &&
+      share(Runs(q, B * T, ldq, 1, 0, (int64_t)n_heads * c.D), Runs(out, B * T, ldo, 1, 0, (int64_t)n_heads * c.D)))
+    return fail(MTTS_E_INVALID, "attention: out overlaps q (in place is fine, with its stride)");
   if (!ws && attn_kv_ws_bytes(B, T, n_heads, c.n_kv, c.D, c.slots, max_len))
     return fail(MTTS_E_INVALID, "attention: workspace required");
   if ((uintptr_t)ws & 15) return fail(MTTS_E_INVALID, "attention: 16-byte aligned workspace");

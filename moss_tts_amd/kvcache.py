@@ -297,7 +297,8 @@ class KVCache:
         """q bf16 [B, T, n_heads, head_dim] of tokens whose keys stand in slots start[b] .. (appended
         before): softmax(scale q . k) v over the context slots that mask (uint8 / bool [B, slots], 1 =
         attend) keeps and the new tokens that tree (int64 [B, T], `tree_masks`; None: a chain) shows.
-        A token that sees nothing gets zeros; rows behind counts[b] are zero, or what `out` held.
+        A token that sees nothing gets zeros; rows behind counts[b] are zero, or what `out` held
+        (`out` is q itself or shares nothing with it).
         max_len: an upper bound of `start` known to the caller, for the shape of the launch only."""
         if q.dim() != 4 or q.dtype is not torch.bfloat16 or q.shape[3] != self.head_dim or q.device != self.device:
             raise ValueError("q: bf16 [B, T, n_heads, head_dim]")

@@ -332,6 +332,20 @@ def test_append_output_is_apart(N, q, k, v, out, ldq, ldkv, ldo, B, S, ok):
     assert append_accepts(N, q, k, v, out, ldq, ldkv, ldo, B, S, 4) == ok
 
 
+@pytest.mark.parametrize("q,ldq,out,ldo,B,T,ok", [
+    (0, 256, 0, 256, 2, 3, True), (0, 512, 0, 512, 2, 3, True),  # in place
+    (0, 256, 256, 256, 2, 3, False), (256, 256, 0, 256, 2, 3, False), (0, 256, 5 * 256, 256, 2, 3, False),
+    (0, 256, 6 * 256, 256, 2, 3, True), (0, 512, 256, 512, 2, 3, True), (0, 512, 128, 512, 2, 3, False),
+    (0, 512, 0, 256, 1, 2, False), (0, 512, 0, 256, 1, 1, True), (0, 256, 64, 256, 1, 1, False),
+    (0, 0, 256, 256, 2, 1, True), (256, 0, 0, 256, 2, 1, False)])
+def test_attention_output_is_apart(N, q, ldq, out, ldo, B, T, ok):
+    """(a workspace that is refused behind the overlap checks keeps the calls from a launch)"""
+    with pytest.raises(ValueError) as e:
+        N.call("mtts_k_attn_kv", ctypes.byref(cache(N)), FAKE + 2 * q, ldq, FAKE + 2 * out, ldo, 4, FAKE, None, None, None, B, T, 0.0, 0,
+               FAKE + 8, None)
+    assert ("workspace" in str(e.value)) == ok and ("overlap" in str(e.value)) != ok
+
+
 def test_output_rows_that_overlap(N):
     c = ctypes.byref(cache(N))
     with pytest.raises(ValueError, match="overlap"):

@@ -607,6 +607,23 @@ def test_rope_outputs_that_share_heads(kv):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("B,T,H,start", [(1, 1, 4, [300]), (2, 6, 4, [9000, 50]), (3, 20, 8, [40, 1300, 0]), (2, 40, 8, [5000, 4000]),
+                                         (2, 150, 6, [90, 600])])
+def test_attend_in_place(kv, kind, B, T, H, start):
+    """out = q is as a new output, in every form, split and not; an output shifted inside q is refused"""
+    g = torch.Generator().manual_seed(T)
+    Hkv, D, S = 2, 64, max(start) + T
+    c = fresh(kv, B, Hkv, S, D, kind)
+    c.write(rnd(g, B, S, Hkv, D).cuda(), rnd(g, B, S, Hkv, D).cuda(), i32([0] * B))
+    buf = rnd(g, B * T * H * D + D).cuda()
+    q, at = buf[:-D].view(B, T, H, D), i32(start)
+    want = c.attend(q, at)
+    with pytest.raises(ValueError, match="overlap"):
+        c.attend(q, at, out=buf[D:].view(B, T, H, D))
+    assert c.attend(q, at, out=q) is q and torch.equal(q, want)
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_nothing_seen_is_zero(kv, kind):
     c = fresh(kv, 2, 1, 256, 64, kind)
     q = torch.ones(2, 3, 2, 64, dtype=torch.bfloat16, device="cuda")
