@@ -309,7 +309,8 @@ int mtts_k_fill_uniform(uint16_t* dst, size_t n, uint64_t seed, uint64_t tensor_
  * over it.  All calls are asynchronous on `stream`, allocate nothing and may be captured into a
  * graph; the caller's current device is the stream's.  Per-row numbers (start, counts, positions,
  * paths, trees) are read on the device: a slot outside 0 .. slots-1 does not exist (nothing is
- * written there or read from there), a count outside 0 .. T is taken as the nearer end. */
+ * written there or read from there), a count outside 0 .. T is taken as the nearer end.  At most 2^25
+ * tokens or slots a row and 2^31 - 1 tokens a call. */
 #define MTTS_KV_BF16 0 /* K [rows][n_kv][slots][D], V transposed [rows][n_kv][D][slots]: the engine's layout */
 #define MTTS_KV_E4M3 1 /* one byte a value, one fp32 scale a (slot, head) for K and for V; 32-slot tiles (kvq.h) */
 #define MTTS_KV_INT8 2

@@ -9,12 +9,14 @@ using namespace mtts;
 
 namespace {
 
+constexpr int KV_SLOTS_MAX = 1 << 25;  // (lane offsets into a cache row are 32 bits of bytes; tile counts round up in 32 bits)
+
 bool view_of(const mtts_kv_cache* c, KvView* v, const char** why) {
   *why = nullptr;
   if (!c || !c->k || !c->v) *why = "cache required";
   else if (c->type != KV_BF16 && c->type != KV_E4M3 && c->type != KV_INT8) *why = "cache type is bf16, e4m3 or int8";
   else if (c->type != KV_BF16 && (!c->k_scale || !c->v_scale)) *why = "an 8-bit cache needs its scales";
-  else if (c->rows < 1 || c->n_kv < 1 || c->slots < 32 || c->slots % 32 || c->slots >= 1 << 25)
+  else if (c->rows < 1 || c->n_kv < 1 || c->slots < 32 || c->slots % 32 || c->slots >= KV_SLOTS_MAX)
     *why = "cache rows, heads and slots (a multiple of 32, below 2^25)";
   else if (((uintptr_t)c->k | (uintptr_t)c->v | (uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & 15)
     *why = "cache pointers are 16-byte aligned";
@@ -181,9 +183,11 @@ extern "C" int mtts_k_kv_append(const mtts_kv_cache* cache, const uint16_t* q, s
   if (B < 0 || B > c.rows || S < 0) return fail(MTTS_E_INVALID, "append: more rows than the cache has");
   if (B == 0 || S == 0) return 0;
   if (!k || !v || !start || (q && (!q_out || n_heads < 1))) return fail(MTTS_E_INVALID, "append: missing arguments");
-  if (q && (int64_t)B * S > 1 && ldqo < (size_t)n_heads * c.D) return fail(MTTS_E_INVALID, "append: rows of q_out overlap");
+  if (S > KV_SLOTS_MAX) return fail(MTTS_E_INVALID, "append: at most 2^25 tokens a row");
+  if (B * (int64_t)S > INT_MAX) return fail(MTTS_E_INVALID, "append: too many tokens");
+  if (q && B * S > 1 && ldqo < (size_t)n_heads * c.D) return fail(MTTS_E_INVALID, "append: rows of q_out overlap");
   // (q may be rotated in place; the heads of other waves and the keys' and values' blocks may not be written)
-  if (q && B * (int64_t)S <= INT_MAX) {
+  if (q) {
     const int M = B * S;
     const Runs o(q_out, M, ldqo, 1, 0, (int64_t)n_heads * c.D);
     if ((!(q == q_out && (M == 1 || ldq == ldqo)) && share(Runs(q, M, ldq, 1, 0, (int64_t)n_heads * c.D), o)) ||
@@ -203,6 +207,7 @@ extern "C" int mtts_k_kv_read(const mtts_kv_cache* cache, uint16_t* k_out, uint1
   if (B == 0 || n == 0) return 0;
   if (!k_out || !v_out || (((uintptr_t)k_out | (uintptr_t)v_out) & 15))
     return fail(MTTS_E_INVALID, "read: 16-byte aligned outputs");
+  if (n > KV_SLOTS_MAX) return fail(MTTS_E_INVALID, "read: at most 2^25 slots");
   HIPCHK(kv_read(KvReadArgs{c, k_out, v_out, start, counts, B, n}, (hipStream_t)stream));
   return 0;
 }
@@ -236,9 +241,9 @@ extern "C" int mtts_k_attn_kv(const mtts_kv_cache* cache, const uint16_t* q, siz
     return fail(MTTS_E_INVALID, "attention: q 16-byte and out 8-byte aligned, in every row; mask and tree 8-byte");
   if ((int64_t)B * T > 1 && ldo < (size_t)n_heads * c.D) return fail(MTTS_E_INVALID, "attention: rows of out overlap");
   if (B > 65535) return fail(MTTS_E_UNSUPPORTED, "attention: at most 65,535 rows");
-  if ((int64_t)T * n_heads > (1 << 30)) return fail(MTTS_E_INVALID, "attention: too many tokens");
+  if ((int64_t)T * n_heads > (1 << 30) || (int64_t)B * T > INT_MAX) return fail(MTTS_E_INVALID, "attention: too many tokens");
   // (a block reads the q of the rows that it writes, before it writes them: in place is fine)
-  if (B * (int64_t)T <= INT_MAX && !(q == out && ((int64_t)B * T == 1 || ldq == ldo)) &&
+  if (!(q == out && (B * T == 1 || ldq == ldo)) &&
       share(Runs(q, B * T, ldq, 1, 0, (int64_t)n_heads * c.D), Runs(out, B * T, ldo, 1, 0, (int64_t)n_heads * c.D)))
     return fail(MTTS_E_INVALID, "attention: out overlaps q (in place is fine, with its stride)");
   if (!ws && attn_kv_ws_bytes(B, T, n_heads, c.n_kv, c.D, c.slots, max_len))

@@ -346,6 +346,28 @@ def test_attention_output_is_apart(N, q, ldq, out, ldo, B, T, ok):
     assert ("workspace" in str(e.value)) == ok and ("overlap" in str(e.value)) != ok
 
 
+BIG = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("n", [BIG, BIG - 30, (1 << 25) + 1])
+def test_sizes_that_pass_the_index_range(N, n):
+    """token and slot counts near 2^31, where rounding up to tiles would pass it"""
+    c = ctypes.byref(cache(N))
+    with pytest.raises(ValueError, match="2\\^25"):
+        N.call("mtts_k_kv_read", c, FAKE, FAKE << 24, None, None, 1, n, None)
+    with pytest.raises(ValueError, match="2\\^25"):
+        N.call("mtts_k_kv_append", c, None, 0, FAKE, 128, FAKE, 128, None, 0, 0, None, None, 0.0, None, None, FAKE, None, 1, n, None)
+
+
+def test_tokens_that_pass_the_index_range(N):
+    many = ctypes.byref(cache(N, rows=128))
+    with pytest.raises(ValueError, match="too many tokens"):
+        N.call("mtts_k_kv_append", many, None, 0, FAKE, 128, FAKE, 128, None, 0, 0, None, None, 0.0, None, None, FAKE, None, 128,
+               1 << 25, None)
+    with pytest.raises(ValueError, match="too many tokens"):
+        N.call("mtts_k_attn_kv", many, FAKE, 256, FAKE, 256, 4, FAKE, None, None, None, 128, 1 << 25, 0.0, 0, FAKE + 8, None)
+
+
 def test_output_rows_that_overlap(N):
     c = ctypes.byref(cache(N))
     with pytest.raises(ValueError, match="overlap"):
