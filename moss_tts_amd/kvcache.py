@@ -324,10 +324,11 @@ class KVCache:
             scale = 0.0
         elif not scale > 0:
             raise ValueError("scale > 0")
+        ld = s1 if T > 1 else s0 if B > 1 else H * D  # (a single token has no stride)
         n = 0 if max_len is None else max(1, int(max_len))
         need = self._f_ws(B, T, H, self.n_kv, D, self.slots, n)
         # (scratch of this call alone, from torch's allocator: in order on this stream, a graph's own in a capture)
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        _call("attend", self._f_attn, self._index, self._ref, q.data_ptr(), s1 if T > 1 else s0, out.data_ptr(), H * D, H,
+        _call("attend", self._f_attn, self._index, self._ref, q.data_ptr(), ld, out.data_ptr(), H * D, H,
               self._start(start, B), self._counts(counts, B), tp, mp, B, T, scale, n, None if ws is None else ws.data_ptr())
         return out

@@ -624,6 +624,18 @@ def test_attend_in_place(kv, kind, B, T, H, start):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+def test_attend_single_token_of_an_odd_row(kv, kind):
+    """one token out of rows of odd length: its address is what counts, there is no next one"""
+    g = torch.Generator().manual_seed(3)
+    c = fresh(kv, 1, 2, 64, 64, kind)
+    c.write(rnd(g, 1, 41, 2, 64).cuda(), rnd(g, 1, 41, 2, 64).cuda(), i32([0]))
+    q = torch.empty(1, 1, 4, 64, dtype=torch.bfloat16, device="cuda").as_strided((1, 1, 4, 64), (259, 259, 64, 1))
+    q.copy_(rnd(g, 1, 1, 4, 64))
+    want = c.attend(q.as_strided((1, 1, 4, 64), (256, 256, 64, 1)), i32([40]))
+    assert q.stride(0) == 259 and torch.equal(c.attend(q, i32([40])), want)
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_nothing_seen_is_zero(kv, kind):
     c = fresh(kv, 2, 1, 256, 64, kind)
     q = torch.ones(2, 3, 2, 64, dtype=torch.bfloat16, device="cuda")
