@@ -378,9 +378,14 @@ int mtts_k_kv_compact(const mtts_kv_cache* cache, const int32_t* start_dev, cons
  * up to 2^100, sums are in 32 bits).  q / out: token b * T + t
  * at + (b * T + t) * ld, [n_heads][head_dim]; rows behind counts[b] are left as they are; out is q with its
  * stride, or shares nothing with it.
- * max_len: an upper bound of start the caller knows (<= 0: slots); it sizes the launch, not the result.
- * ws_dev: mtts_k_attn_kv_ws_bytes bytes of scratch (0: NULL is fine), not shared by calls that may run
- * at once; nothing is kept in it.  At most 65,535 rows. */
+ * max_len: an upper bound of start the caller knows (<= 0: slots); it sizes the launch, and a wrong one
+ * costs time alone.  ws_dev: mtts_k_attn_kv_ws_bytes bytes of scratch (0: NULL is fine), not shared by calls
+ * that may run at once; nothing is kept in it.  At most 65,535 rows.
+ * The same call gives the same bits.  Where the workspace is 0 bytes a row's bits do not depend on the
+ * other rows' lengths or values; elsewhere long rows are cut where the lengths of all rows put the cuts, and
+ * a row's rounding moves with them, as it does with B, T and max_len.  Probabilities are rounded to bf16; their
+ * sum is that of the rounded ones, but for 8-bit caches above 32 rows (T n_heads / n_kv) a KV head, where it is
+ * that of the values before (a result is off by 0.0024 of its size there, and by 0.0019 elsewhere). */
 size_t mtts_k_attn_kv_ws_bytes(int B, int T, int n_heads, int n_kv, int head_dim, int slots, int max_len);
 int mtts_k_attn_kv(const mtts_kv_cache* cache, const uint16_t* q, size_t ldq, uint16_t* out, size_t ldo, int n_heads,
                    const int32_t* start_dev, const int32_t* counts_dev, const uint64_t* tree_dev, const uint8_t* mask_dev,

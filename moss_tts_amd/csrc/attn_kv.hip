@@ -45,6 +45,8 @@ __device__ __forceinline__ RowLen row_len(const AttnKvArgs& a, int b) {
 // 2 x if it began before, and the join adds them up in order: the first block and the number of blocks of
 // each row stand at the head of the workspace.  share 0: a block a row, nothing to join.
 // A segment more costs a block about SEG tiles (its loads start anew), so a row counts for SEG more.
+// Where a row is cut follows from the lengths of all rows, and so do the maxima that its parts start with and
+// the last bits of its result (cuts that each row had for itself would leave the blocks uneven).
 __device__ __forceinline__ int tiles_of(const RowLen& r) { return r.n ? max(1, (r.nk + 31) >> 5) : 0; }
 // sum up to and with this lane: rows of 16 lanes by shifts, then the rows' sums by broadcasts
 __device__ __forceinline__ int wave_iscan(int v) {

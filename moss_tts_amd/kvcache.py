@@ -299,7 +299,9 @@ class KVCache:
         attend) keeps and the new tokens that tree (int64 [B, T], `tree_masks`; None: a chain) shows.
         A token that sees nothing gets zeros; rows behind counts[b] are zero, or what `out` held
         (`out` is q itself or shares nothing with it).
-        max_len: an upper bound of `start` known to the caller, for the shape of the launch only."""
+        max_len: an upper bound of `start` known to the caller, for the shape of the launch.  The same
+        call gives the same bits; a long row's rounding may differ beside rows of other lengths, or with
+        another max_len."""
         if q.dim() != 4 or q.dtype is not torch.bfloat16 or q.shape[3] != self.head_dim or q.device != self.device:
             raise ValueError("q: bf16 [B, T, n_heads, head_dim]")
         B, T, H, D = q.shape

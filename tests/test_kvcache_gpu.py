@@ -494,6 +494,35 @@ def test_attend_many_short_rows(kv, kind, B, T, H, Hkv):
                 counts=[T - b % 3 if b % 11 else 0 for b in range(B)])
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T,H,split", [(1, 8, False), (12, 8, False), (30, 8, False), (64, 8, False), (1, 8, True), (12, 8, True),
+                                       (64, 8, True)])
+def test_rows_beside_other_rows(kv, kind, T, H, split):
+    """A row beside others of other lengths and contents.  Without a workspace its bits are the same; with one,
+    long rows are cut where the lengths of all rows put the cuts: the same within rounding, and the same bits for
+    the same call"""
+    from moss_tts_amd import _native as N
+    g = torch.Generator().manual_seed(T)
+    Hkv, D, B, slots, n = 2, 64, 3, 6080 if split else 512, 5000 if split else 400
+    assert (N.load().mtts_k_attn_kv_ws_bytes(B, T, H, Hkv, D, slots, 0) > 0) == split
+    k, v, q = rnd(g, B, slots, Hkv, D).cuda(), rnd(g, B, slots, Hkv, D).cuda(), rnd(g, B, T, H, D).cuda()
+    outs = []
+    for other in ([0, 0], [17, 33], [slots - T, 100], [40, slots]):
+        c = fresh(kv, B, Hkv, slots, D, kind)
+        c.write(k, v, i32([0] * B))
+        for max_len in (None, slots):
+            outs.append(c.attend(q, i32([other[0], n, other[1]]), max_len=max_len)[1].clone())
+        assert torch.equal(outs[-1], c.attend(q, i32([other[0], n, other[1]]), max_len=slots)[1])
+        k[[0, 2]], v[[0, 2]], q[[0, 2]] = -k[[0, 2]] * 3, v[[0, 2]] + 1, q[[2, 0]]
+    if not split:
+        assert all(torch.equal(x, outs[0]) for x in outs)
+    see = sees(B, T, slots, [0, n, 0], None, None, None)[1:2]
+    from tests.kv_layout import contents
+    ck, cv = (x[1:2] for x in contents(c))
+    for x in outs:
+        attention_close(x[None].cpu(), *attend64(q[1:2].cpu(), ck, cv, see, D ** -0.5), D)
+
+
 def test_two_streams_at_once(kv):
     """calls of two streams over one cache, each with a workspace of its own, as one after the other"""
     g = torch.Generator().manual_seed(11)
