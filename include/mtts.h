@@ -385,7 +385,8 @@ int mtts_k_kv_compact(const mtts_kv_cache* cache, const int32_t* start_dev, cons
  * other rows' lengths or values; elsewhere long rows are cut where the lengths of all rows put the cuts, and
  * a row's rounding moves with them, as it does with B, T and max_len.  Probabilities are rounded to bf16; their
  * sum is that of the rounded ones, but for 8-bit caches above 32 rows (T n_heads / n_kv) a KV head, where it is
- * that of the values before (a result is off by 0.0024 of its size there, and by 0.0019 elsewhere). */
+ * that of the values before.  (Results are off by 0.0017 to 0.0025 of their size; where one key takes
+ * nearly all, by about 0.003 there and 0.002 elsewhere.) */
 size_t mtts_k_attn_kv_ws_bytes(int B, int T, int n_heads, int n_kv, int head_dim, int slots, int max_len);
 int mtts_k_attn_kv(const mtts_kv_cache* cache, const uint16_t* q, size_t ldq, uint16_t* out, size_t ldo, int n_heads,
                    const int32_t* start_dev, const int32_t* counts_dev, const uint64_t* tree_dev, const uint8_t* mask_dev,

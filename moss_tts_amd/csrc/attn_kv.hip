@@ -128,7 +128,7 @@ struct Segments {
 };
 // f of each segment of block x.  Unsplit launches (SPLIT false) have a kernel of their own: with the sharing
 // out in it too it is twice the code, whose fetching a short call waits for (one token over 389 bf16 slots
-// 10.3 us and not 8), and the loop over 32 rows of 4,000 slots took 94 us and not 81.
+// 10.3 us and not 8), and the loop over 32 rows of 2,063 to 4,000 slots took 94 us and not 81.
 template <bool SPLIT, int SEG, class F>
 __device__ __forceinline__ void for_segments(const AttnKvArgs& a, int NS, int least, int x, bool head, F&& f) {
   if constexpr (SPLIT) {
@@ -306,7 +306,8 @@ struct RowState {
   // product's type: half a step of 2^-8 at random signs over the keys.  l sums the rounded values, so that
   // a key that takes nearly all keeps nearly all of 1, whatever its rounding (8-bit types: with COMP, which
   // costs 16 more instructions a tile, nothing to 1 us of 42 where the cache's bytes are the bound; without,
-  // the values before rounding).  Sums stay in 32 bits.
+  // the values before rounding: one key at 0.987, the output is off by 0.0018 with it and 0.0030 without).  Sums
+  // stay in 32 bits.
   template <bool COMP>
   __device__ __forceinline__ void probs(const f32x16& s, float c, float vsl, uint32_t sees, bool special, bf16x8* p) {
     constexpr bool Q8 = KT != KV_BF16;
@@ -582,10 +583,12 @@ __device__ __forceinline__ void merge_groups(const AttnKvArgs& a, int b, int hkv
 // block take tiles in turn, loaded one tile ahead, with no barrier in the loop, and merge once at the
 // end.  8-bit fragments go from memory straight into registers, bf16 ones through LDS of the wave's own
 // (straight, a wave-wide load of them touched 64 lines of memory).
-//   Measured with 32 q heads on 8 KV heads of 128, one token a row: 32 rows of 4,000 slots bf16 81 us
-// (4.9 TB/s), e4m3 41 us (5.0 TB/s); one row of 130,000 bf16 114 us (4.7 TB/s, with the join), e4m3 66 us
-// (4.2 TB/s); a large copy reaches 4.9.  One row of 389 bf16 slots 8 us: a chain of dependent loads
-// (length, tiles, merge) and the first fetch of 20 KB of code.
+//   Measured with 32 q heads on 8 KV heads of 128, one token a row, without a mask: 32 rows of 4,000 slots
+// bf16 93 us (5.7 TB/s), e4m3 48 us (5.7 TB/s), rows of 2,063 to 4,000 slots 80 and 40 us (5.0 and 5.1 TB/s:
+// the long rows' blocks end last); one row of 130,000 bf16 111 us (4.8 TB/s, with the join), e4m3 69 us
+// (4.0 TB/s); a large copy reaches 4.9.  One row of 389 bf16 slots 8 us: a chain of dependent loads
+// (length, tiles, merge) and the first fetch of 20 KB of code.  A mask makes an edge tile of every tile, and its
+// bytes are waited for inside the turn, with the tiles in flight.
 template <int KT, int D, int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, 2) void attn_kv_keys(AttnKvArgs a, int NS, int least, uint32_t rG) {
   constexpr bool Q8 = KT != KV_BF16;
@@ -741,16 +744,18 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_kv_keys(AttnKvArgs a, int NS,
   });
 }
 
-// More rows: bound by the arithmetic on the scores (of a tile's turn the products take half, the powers, the
-// maximum and the roundings the rest, and two waves a SIMD hide little of one behind the other).  W waves,
+// More rows: bound by the arithmetic on the scores (of a tile's turn the products take about a third, the powers,
+// the maximum and the roundings the rest, and two waves a SIMD hide little of one behind the other).  W waves,
 // 32 rows each, go through the same tiles, whose fragments they load, turn into bf16 and put into LDS
 // together, once for all rows, a turn ahead of the products (two halves of LDS, one barrier a turn).
 //   A block has KS such groups, which take the tiles in turn and are merged at the end: with a block each
-// (KS 1), four or two times the partials went through memory: 4 rows of 7,500 e4m3 slots and 16 tokens of
-// 4 heads wrote and read 32 MB of them beside the cache's 50 MB (42 us, 36 like this).
-//   Measured with 32 q heads on 8 KV heads of 128: one row of 130,001 int8 slots, 33 tokens, 160 us
-// (440 TFLOP/s; three of the eight waves have no rows there), 16 rows of 4,000 bf16 slots, 64 tokens, 73 us
-// and 12 for the join (610 TFLOP/s); a large plain matrix product reaches 1,150.
+// (KS 1), four or two times the partials went through memory: 4 rows of 4,688 to 7,500 e4m3 slots and 16 tokens
+// of 4 heads wrote and read 32 MB of them beside the cache's 50 MB (42 us, 36 like this; left pads).
+//   Measured with 32 q heads on 8 KV heads of 128, without a mask: one row of 130,001 slots, 33 tokens, bf16
+// 137 us, e4m3 141, int8 151 (510, 500, 470 TFLOP/s; three of the eight waves have no rows there); 16 rows of
+// 4,000 slots, 64 tokens, 97, 97, 100 (700, 710, 680 TFLOP/s; of it 12 us the join); a large plain matrix
+// product reaches 1,150.  4 rows of 7,500 slots, 16 tokens: 39, 27, 28, and 54, 39, 39 with a mask, for which
+// every tile is an edge tile: two looks at its bytes, the selects, and a wait for the tiles in flight.
 template <int KT, int D, int W, int KS>
 __global__ __launch_bounds__(64 * W * KS, 2) void attn_kv_rows(AttnKvArgs a, int NS, int least, int RB) {
   constexpr bool Q8 = KT != KV_BF16;
@@ -1012,8 +1017,9 @@ struct AkvPlan {
   int W, RB, NS, least;
 };
 // Constants by measurement, 32 q heads on 8 KV heads of 128, bf16 / e4m3, us:
-//   form: one tile of rows stays with its waves' registers (keys); two as groups of two waves, .. (a group's
-//     rows are a power of two of tiles, so that the tile's loads divide among its waves);
+//   (rows of a batch: from the slots given down to about half of them)
+//   form: one tile of rows stays with its waves' registers (keys); more go to the next of the groups that are
+//     built, of two, four or eight waves: those beyond the rows' tiles help with the loads alone;
 //   least (tiles a block): 1 row, 16 tokens, 2,000 slots: 8 19.2 / 19.0, 16 21.8 / 21.4; W 8 has no groups
 //     that share a block's tiles: 4;
 //   most (tiles up to which nothing is split): W 2, 1 row of 500 slots: 16 19.6 / 19.4, 32 17.8 / 16.5;

@@ -193,9 +193,10 @@ __device__ __forceinline__ int row_count(const int* counts, int b, int S) {
 //   [.., +nk)  k: a block per (row, kv head, tile of 32 slots): norm, rotation, amax over the head's lanes,
 //              codes through LDS into the tile's order, so that they leave in 16-byte pieces side by side
 //   [.., +nk)  v: the same; a V tile holds 16 slots of one dim side by side
-// One launch, so that a decode step pays once.  Bound by its bytes: 3 rows of 2,117 tokens, 32 q and 16 k and
-// v heads of 128, to e4m3: 143 MB in 33 us (4.3 TB/s; the rows' last tiles and the norm's second look at
-// its lanes are the rest); one token 5.5 us, of which the chain load, sum, angle, amax, store is most.
+// One launch, so that a decode step pays once.  Rows of 2,117, 1,882 and 1,647 tokens, 32 q and 8 + 8 k and v
+// heads of 128, to e4m3: 128 MB in 33.4 us (3.8 TB/s, where a large copy reaches 4.9; each K block computes
+// its tokens' angles in 64 bits, their sines and cosines for its own KV head, so 8 times in all, and the rows'
+// last tiles are partly empty); one token 5.4 us, of which the chain load, sum, angle, amax, store is most.
 template <int V>
 __device__ __forceinline__ float head_sum(float s, int pt) {
   for (int o = 1; o < pt; o <<= 1) s += __shfl_xor(s, o, 64);
@@ -521,8 +522,9 @@ hipError_t kv_read(const KvReadArgs& a, hipStream_t s) {
 // in any order.  An entry whose source or destination is no slot is left out.  K moves in 16-byte pieces.
 // V has its slots side by side, so the window of slots that a path can touch goes through LDS in 16-byte
 // pieces (a piece at an edge writes the slots beside the window back as they were): byte by byte, 64 rows
-// of 64 tokens took 14.5 us; they take 8.6 (8 int8 heads of 128; 1 row of 16 tokens 4.3, two dependent loads
-// and a launch).
+// of 64 tokens took 14.5 us; they take 9.2 (8 int8 heads of 128, about half of the tokens kept; the window is
+// read and written whatever the path is, in one dependent chain a block).  1 row of 16 tokens 4.4, two
+// dependent loads and a launch.
 constexpr int KV_WIN = KV_PATH_MAX + 32;  // slots of the window: whole tiles (8-bit), or pieces of 8 (bf16)
 __global__ __launch_bounds__(256) void kv_compact_kernel(KvCompactArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t win[KV_DMAX * (KV_PATH_MAX + 8) * 2];
