@@ -107,6 +107,7 @@ class Rope:
         _need(head_dim >= 2 and head_dim % 2 == 0, "head_dim is even")
         _need(2 <= self.rotary_dim <= head_dim and self.rotary_dim % 2 == 0, "rotary_dim is even and at most head_dim")
         if inv_freq is None:
+            _need(factor == 1.0, "factor goes with inv_freq; a scaling has its own")
             turns, self.factor = rope_turns(self.rotary_dim, theta, scaling)
         else:
             _need(scaling is None and inv_freq.numel() == self.rotary_dim // 2,

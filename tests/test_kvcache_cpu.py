@@ -150,6 +150,13 @@ def test_rope_explicit_values_are_used(kv):
         assert abs(factor - m) <= 2.0 ** -24 * m
 
 
+@pytest.mark.parametrize("kw", [dict(factor=2.0), dict(factor=2.0, scaling=YARN), dict(factor=NAN)])
+def test_rope_factor_without_frequencies(kv, kw):
+    """a factor that would not be applied is refused (before a device is looked for)"""
+    with pytest.raises(ValueError, match="factor"):
+        kv.Rope(64, **kw)
+
+
 def test_tree_masks(kv):
     masks, depth = kv.tree_masks([[-1, 0, 0, 1, 3], [-1, -1, 1, 2, 0]])
     assert masks.tolist() == [[1, 3, 5, 11, 27], [1, 2, 6, 14, 17]]
