@@ -356,7 +356,8 @@ int mtts_k_rope(const uint16_t* x, size_t ldx, size_t hsx, uint16_t* y, size_t l
  * norm (qn_w) and rotation, to q_out in bf16; rows behind counts[b] are left as they are.  q_out is q with
  * its stride, or shares nothing with q, k and v.
  * A head's values are stored as code * scale, scale = max|x| / Q, code = nearest(x Q / max|x|), Q = 448
- * (e4m3) or 127 (int8); a head below 2^-100 as zeros, one with a NaN or an infinity as NaN in whole. */
+ * (e4m3) or 127 (int8); a head below 2^-100 as zeros, one with a NaN or an infinity as NaN in whole.  The
+ * norm's sum of squares is held in 32 bits: values up to 2^60. */
 int mtts_k_kv_append(const mtts_kv_cache* cache, const uint16_t* q, size_t ldq, const uint16_t* k, size_t ldk,
                      const uint16_t* v, size_t ldv, uint16_t* q_out, size_t ldqo, int n_heads, const uint16_t* qn_w,
                      const uint16_t* kn_w, float eps, const mtts_rope* rope, const int32_t* pos_dev,
