@@ -354,7 +354,7 @@ int mtts_k_rope(const uint16_t* x, size_t ldx, size_t hsx, uint16_t* y, size_t l
  * in one packed row).  k: RMSNorm over the head with weight kn_w (NULL: none), rotation (rope NULL:
  * none) at pos_dev [B * S] (NULL: the slot), then quantised; v: quantised.  q (NULL: none): the same
  * norm (qn_w) and rotation, to q_out in bf16; rows behind counts[b] are left as they are.  q_out is q with
- * its stride, or shares nothing with q, k and v.
+ * its stride, or shares nothing with q, k and v; k and v lie outside the cache.
  * A head's values are stored as code * scale, scale = max|x| / Q, code = nearest(x Q / max|x|), Q = 448
  * (e4m3) or 127 (int8); a head below 2^-100 as zeros, one with a NaN or an infinity as NaN in whole.  The
  * norm's sum of squares is held in 32 bits: values up to 2^60. */

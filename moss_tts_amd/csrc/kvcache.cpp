@@ -186,6 +186,12 @@ extern "C" int mtts_k_kv_append(const mtts_kv_cache* cache, const uint16_t* q, s
   if (S > KV_SLOTS_MAX) return fail(MTTS_E_INVALID, "append: at most 2^25 tokens a row");
   if (B * (int64_t)S > INT_MAX) return fail(MTTS_E_INVALID, "append: too many tokens");
   if (q && B * S > 1 && ldqo < (size_t)n_heads * c.D) return fail(MTTS_E_INVALID, "append: rows of q_out overlap");
+  // (where its slots are is known on the device alone)
+  const int64_t held = (int64_t)(mtts_kv_bytes(c.type, c.rows, c.n_kv, c.D, c.slots) / 2);
+  for (const void* buf : {c.k, c.v})
+    for (const auto& [src, ld] : {std::pair<const uint16_t*, size_t>(k, ldk), {v, ldv}})
+      if (share(Runs(src, B * S, ld, 1, 0, (int64_t)c.n_kv * c.D), Runs(buf, 1, 0, 1, 0, held)))
+        return fail(MTTS_E_INVALID, "append: k and v lie outside the cache");
   // (q may be rotated in place; the heads of other waves and the keys' and values' blocks may not be written)
   if (q) {
     const int M = B * S;

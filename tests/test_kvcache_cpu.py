@@ -318,7 +318,7 @@ def test_rope_overlap_is_exact(N):
 def append_accepts(N, q, k, v, out, ldq, ldkv, ldo, B, S, H):
     """as rope_accepts; 2 KV heads of 64"""
     with pytest.raises(ValueError) as e:
-        N.call("mtts_k_kv_append", ctypes.byref(cache(N)), FAKE + 2 * q, ldq, FAKE + 2 * k, ldkv, FAKE + 2 * v, ldkv, FAKE + 2 * out,
+        N.call("mtts_k_kv_append", ctypes.byref(cache(N, k=FAKE << 8, v=FAKE << 9)), FAKE + 2 * q, ldq, FAKE + 2 * k, ldkv, FAKE + 2 * v, ldkv, FAKE + 2 * out,
                ldo, H, None, None, 0.0, ctypes.byref(N.MttsRope(FAKE, 3, 0, 1.0)), None, FAKE, None, B, S, None)
     assert "overlap" in str(e.value) or "rotary" in str(e.value)
     return "overlap" not in str(e.value)
@@ -373,6 +373,19 @@ def test_tokens_that_pass_the_index_range(N):
                1 << 25, None)
     with pytest.raises(ValueError, match="too many tokens"):
         N.call("mtts_k_attn_kv", many, FAKE, 256, FAKE, 256, 4, FAKE, None, None, None, 128, 1 << 25, 0.0, 0, FAKE + 8, None)
+
+
+@pytest.mark.parametrize("k,v,ld,ok", [(0, 1 << 20, 128, False), (1 << 20, 0, 128, False), (32767, 1 << 20, 128, False),
+                                       (1 << 20, 49151, 128, False), (49152, 16384, 128, True), (65536, 1 << 20, 128, True),
+                                       (-256, 1 << 20, 128, True), (-255, 1 << 20, 128, False), (-128, 1 << 20, 20000, True)])
+def test_append_from_the_cache_itself(N, k, v, ld, ok):
+    """keys or values that lie in the cache would be read while their slots are written; 2 rows x 2 heads x
+    64 slots x 64 bf16: K's 16,384 values at 0, V's at 32,768"""
+    c = cache(N, type=0, k=FAKE << 8, v=(FAKE << 8) + 65536, k_scale=None, v_scale=None)
+    with pytest.raises(ValueError) as e:
+        N.call("mtts_k_kv_append", ctypes.byref(c), None, 0, (FAKE << 8) + 2 * k, ld, (FAKE << 8) + 2 * v, ld, None, 0, 0, None, None, 0.0,
+               ctypes.byref(N.MttsRope(FAKE, 3, 0, 1.0)), None, FAKE, None, 1, 2, None)
+    assert ("rotary" in str(e.value)) == ok and ("cache" in str(e.value)) != ok
 
 
 def test_output_rows_that_overlap(N):
